@@ -7,7 +7,7 @@ hand-written gfx950 HIP kernels in libffa.so (C ABI: include/ffa.h).
 """
 
 from .config import AttentionConfig
-from .modules import FastestFlashGQA, FastestFlashMHA, FastestFlashMLA
+from .modules import FastestFlashGQA, FastestFlashMHA, FastestFlashMLA, FastestFlashRotary
 from .ops import (
     ContinuousKVCache,
     FastestFlashAttnFunc,
@@ -20,8 +20,13 @@ from .ops import (
     fastest_flash_attn_backward,
     fastest_flash_attn_forward,
     fastest_flash_attn_func,
+    fastest_flash_copy_pages,
     fastest_flash_mla_decode,
+    fastest_flash_paged_append,
     fastest_flash_paged_decode,
+    fastest_flash_rotary,
+    rotary_frequencies,
+    yarn_magnitude,
 )
 from .utils import auto_select_block_size, check_hip_available, check_triton_available
 
@@ -34,11 +39,17 @@ __all__ = [
     "fastest_flash_attn_func",
     "FastestFlashAttnFunc",
     "fastest_flash_paged_decode",
+    "fastest_flash_paged_append",
+    "fastest_flash_copy_pages",
+    "fastest_flash_rotary",
+    "rotary_frequencies",
+    "yarn_magnitude",
     "fastest_flash_mla_decode",
     "MLALatentCache",
     "FastestFlashMHA",
     "FastestFlashGQA",
     "FastestFlashMLA",
+    "FastestFlashRotary",
     "PagedKVCache",
     "ContinuousKVCache",
     "create_causal_block_mask",

@@ -20,7 +20,7 @@ import torch  # noqa: F401  (must load torch's HIP runtime before libffa.so)
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libffa.so")
 
-FFA_ABI_VERSION = 13
+FFA_ABI_VERSION = 14
 FFA_DTYPE_BF16 = 0
 FFA_DTYPE_FP16 = 1
 FFA_DTYPE_FP32 = 2
@@ -238,6 +238,83 @@ class MlaAssembleArgs(ctypes.Structure):
     ]
 
 
+class RotaryArgs(ctypes.Structure):
+    """Mirror of ``ffa_rotary_args``."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("q_out", ctypes.c_void_p),
+        ("k_out", ctypes.c_void_p),
+        ("inv_freq", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("q_stride", _I64x3),
+        ("k_stride", _I64x3),
+        ("q_out_stride", _I64x3),
+        ("k_out_stride", _I64x3),
+        ("position_stride", _I64x2),
+        ("q_offset", ctypes.c_int64),
+        ("batch", ctypes.c_int32),
+        ("heads_q", ctypes.c_int32),
+        ("heads_k", ctypes.c_int32),
+        ("seqlen", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("rotary_dim", ctypes.c_int32),
+        ("position_bytes", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("inverse", ctypes.c_int32),
+        ("magnitude", ctypes.c_float),
+        ("dtype", ctypes.c_int32),
+    ]
+
+
+class PagedAppendBatchArgs(ctypes.Structure):
+    """Mirror of ``ffa_paged_append_batch_args``."""
+
+    _fields_ = [
+        ("k_pages", ctypes.c_void_p),
+        ("v_pages", ctypes.c_void_p),
+        ("k_new", ctypes.c_void_p),
+        ("v_new", ctypes.c_void_p),
+        ("q", ctypes.c_void_p),
+        ("q_out", ctypes.c_void_p),
+        ("inv_freq", ctypes.c_void_p),
+        ("block_tables", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("counts", ctypes.c_void_p),
+        ("k_new_stride", _I64x3),
+        ("v_new_stride", _I64x3),
+        ("q_stride", _I64x3),
+        ("q_out_stride", _I64x3),
+        ("block_table_stride", ctypes.c_int32),
+        ("batch", ctypes.c_int32),
+        ("heads_q", ctypes.c_int32),
+        ("heads_kv", ctypes.c_int32),
+        ("n_tokens", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("rotary_dim", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("magnitude", ctypes.c_float),
+        ("dtype", ctypes.c_int32),
+    ]
+
+
+class PagedCopyArgs(ctypes.Structure):
+    """Mirror of ``ffa_paged_copy_args``."""
+
+    _fields_ = [
+        ("k_pages", ctypes.c_void_p),
+        ("v_pages", ctypes.c_void_p),
+        ("src", ctypes.c_void_p),
+        ("dst", ctypes.c_void_p),
+        ("page_bytes", ctypes.c_int64),
+        ("n_pairs", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32),
+    ]
+
+
 class AttnBwdArgs(ctypes.Structure):
     """Mirror of ``ffa_attn_bwd_args``."""
 
@@ -301,6 +378,11 @@ EXPORTS = {
     "ffa_mla_decode_fwd": (ctypes.c_int, [ctypes.POINTER(MlaDecodeArgs), ctypes.c_void_p]),
     "ffa_rope_tables": (ctypes.c_int, [ctypes.POINTER(RopeTablesArgs), ctypes.c_void_p]),
     "ffa_mla_assemble": (ctypes.c_int, [ctypes.POINTER(MlaAssembleArgs), ctypes.c_void_p]),
+    "ffa_rotary": (ctypes.c_int, [ctypes.POINTER(RotaryArgs), ctypes.c_void_p]),
+    "ffa_paged_append_batch": (
+        ctypes.c_int, [ctypes.POINTER(PagedAppendBatchArgs), ctypes.c_void_p],
+    ),
+    "ffa_paged_copy": (ctypes.c_int, [ctypes.POINTER(PagedCopyArgs), ctypes.c_void_p]),
     "ffa_attn_bwd_workspace_bytes": (
         ctypes.c_size_t, [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32],
     ),

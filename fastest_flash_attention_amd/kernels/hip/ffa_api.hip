@@ -26,6 +26,11 @@ int check_v_head_dim(int32_t v_head_dim, int32_t head_dim, int32_t dtype) {
   return v_head_dim % 8 != 0 ? FFA_ERR_MISALIGNED : FFA_OK;
 }
 
+// rotary_dim: even, within the head. magnitude: finite.
+bool valid_rotary(int32_t rotary_dim, int32_t head_dim, float magnitude) {
+  return rotary_dim >= 0 && rotary_dim % 2 == 0 && rotary_dim <= head_dim && std::isfinite(magnitude);
+}
+
 // scale: any finite value. softcap: <= 0 (none) or a finite positive cap.
 bool valid_scale(float scale, float softcap) {
   return std::isfinite(scale) && !std::isnan(softcap) && !(softcap > 0.0f && std::isinf(softcap));
@@ -380,6 +385,85 @@ int ffa_mla_assemble(const ffa_mla_assemble_args* a, void* stream) {
     if (st % 8 != 0) return FFA_ERR_MISALIGNED;
   }
   return ffa::launch_mla_assemble(*a, static_cast<hipStream_t>(stream));
+}
+
+int ffa_rotary(const ffa_rotary_args* a, void* stream) {
+  if (a == nullptr) return FFA_ERR_INVALID_ARG;
+  if (!valid_dtype(a->dtype) && a->dtype != FFA_DTYPE_FP32) return FFA_ERR_UNSUPPORTED_DTYPE;
+  if (a->batch < 0 || a->heads_q < 0 || a->heads_k < 0 || a->seqlen < 0 || a->head_dim < 1 ||
+      !valid_rotary(a->rotary_dim, a->head_dim, a->magnitude) || a->rotary_dim < 2) {
+    return FFA_ERR_INVALID_ARG;
+  }
+  if (a->batch == 0 || a->seqlen == 0) return FFA_OK;
+  if (a->inv_freq == nullptr || (a->heads_q > 0 && (a->q == nullptr || a->q_out == nullptr)) ||
+      (a->heads_k > 0 && (a->k == nullptr || a->k_out == nullptr))) {
+    return FFA_ERR_INVALID_ARG;
+  }
+  for (int i = 0; i < 3; ++i) {
+    if (a->q_stride[i] < 0 || a->k_stride[i] < 0 || a->q_out_stride[i] < 0 || a->k_out_stride[i] < 0) {
+      return FFA_ERR_INVALID_ARG;
+    }
+  }
+  const uintptr_t unit = a->dtype == FFA_DTYPE_FP32 ? 4 : 2;
+  const void* ptrs[4] = {a->heads_q > 0 ? a->q : nullptr, a->heads_q > 0 ? a->q_out : nullptr,
+                         a->heads_k > 0 ? a->k : nullptr, a->heads_k > 0 ? a->k_out : nullptr};
+  for (const void* ptr : ptrs) {
+    if (reinterpret_cast<uintptr_t>(ptr) % unit != 0) return FFA_ERR_MISALIGNED;
+  }
+  if (reinterpret_cast<uintptr_t>(a->inv_freq) % 8 != 0) return FFA_ERR_MISALIGNED;
+  if (a->positions != nullptr) {
+    if (a->position_bytes != 4 && a->position_bytes != 8) return FFA_ERR_INVALID_ARG;
+    if (a->position_stride[0] < 0 || a->position_stride[1] < 0) return FFA_ERR_INVALID_ARG;
+    if (reinterpret_cast<uintptr_t>(a->positions) % a->position_bytes != 0) return FFA_ERR_MISALIGNED;
+  }
+  return ffa::launch_rotary(*a, static_cast<hipStream_t>(stream));
+}
+
+int ffa_paged_append_batch(const ffa_paged_append_batch_args* a, void* stream) {
+  if (a == nullptr) return FFA_ERR_INVALID_ARG;
+  if (!valid_dtype(a->dtype) && a->dtype != FFA_DTYPE_FP32) return FFA_ERR_UNSUPPORTED_DTYPE;
+  if (a->batch < 0 || a->heads_q < 0 || a->heads_kv < 1 || a->n_tokens < 0 || a->head_dim < 1 ||
+      a->page_size < 1 || a->num_pages < 0 || a->block_table_stride < 0 ||
+      !valid_rotary(a->rotary_dim, a->head_dim, a->magnitude)) {
+    return FFA_ERR_INVALID_ARG;
+  }
+  if (a->batch == 0 || a->n_tokens == 0) return FFA_OK;
+  if (a->k_pages == nullptr || a->v_pages == nullptr || a->k_new == nullptr || a->v_new == nullptr ||
+      a->block_tables == nullptr || a->positions == nullptr ||
+      (a->rotary_dim > 0 && a->inv_freq == nullptr) ||
+      (a->heads_q > 0 && (a->q == nullptr || a->q_out == nullptr))) {
+    return FFA_ERR_INVALID_ARG;
+  }
+  for (int i = 0; i < 3; ++i) {
+    if (a->k_new_stride[i] < 0 || a->v_new_stride[i] < 0 || a->q_stride[i] < 0 || a->q_out_stride[i] < 0) {
+      return FFA_ERR_INVALID_ARG;
+    }
+  }
+  const uintptr_t unit = a->dtype == FFA_DTYPE_FP32 ? 4 : 2;
+  const void* ptrs[6] = {a->k_pages, a->v_pages, a->k_new, a->v_new, a->heads_q > 0 ? a->q : nullptr,
+                         a->heads_q > 0 ? a->q_out : nullptr};
+  for (const void* ptr : ptrs) {
+    if (reinterpret_cast<uintptr_t>(ptr) % unit != 0) return FFA_ERR_MISALIGNED;
+  }
+  const void* ints[3] = {a->block_tables, a->positions, a->counts};
+  for (const void* ptr : ints) {
+    if (reinterpret_cast<uintptr_t>(ptr) % 4 != 0) return FFA_ERR_MISALIGNED;
+  }
+  if (a->rotary_dim > 0 && reinterpret_cast<uintptr_t>(a->inv_freq) % 8 != 0) return FFA_ERR_MISALIGNED;
+  return ffa::launch_paged_append_batch(*a, static_cast<hipStream_t>(stream));
+}
+
+int ffa_paged_copy(const ffa_paged_copy_args* a, void* stream) {
+  if (a == nullptr || a->n_pairs < 0 || a->num_pages < 0 || a->page_bytes < 0) return FFA_ERR_INVALID_ARG;
+  if (a->n_pairs == 0 || a->page_bytes == 0) return FFA_OK;
+  if (a->k_pages == nullptr || a->src == nullptr || a->dst == nullptr) return FFA_ERR_INVALID_ARG;
+  const uint64_t bits = reinterpret_cast<uintptr_t>(a->k_pages) | reinterpret_cast<uintptr_t>(a->v_pages) |
+                        static_cast<uint64_t>(a->page_bytes);
+  if (bits % 2 != 0 || reinterpret_cast<uintptr_t>(a->src) % 4 != 0 ||
+      reinterpret_cast<uintptr_t>(a->dst) % 4 != 0) {
+    return FFA_ERR_MISALIGNED;
+  }
+  return ffa::launch_paged_copy(*a, static_cast<hipStream_t>(stream));
 }
 
 size_t ffa_attn_bwd_workspace_bytes(int32_t batch, int32_t heads_q, int32_t seqlen_q) {

@@ -47,4 +47,12 @@ int launch_attn_bwd(const ffa_attn_bwd_args& a, hipStream_t stream);
 int launch_paged_gather(const ffa_paged_gather_args& a, hipStream_t stream);
 int launch_paged_append(const ffa_paged_append_args& a, hipStream_t stream);
 
+
+// Rotary positions, and a batch's new tokens into the paged pools.
+int launch_rotary(const ffa_rotary_args& a, hipStream_t stream);
+int launch_paged_append_batch(const ffa_paged_append_batch_args& a, hipStream_t stream);
+
+// Page copies.
+int launch_paged_copy(const ffa_paged_copy_args& a, hipStream_t stream);
+
 }  // namespace ffa

@@ -11,6 +11,9 @@ then the S new K/V rows are repeated to ``num_heads`` as the reference repeats t
 the op runs with one KV head per q head. A cache of ``num_kv_heads`` heads is accepted
 too (an extension: it is what the unrepeated path concatenates with, and it is
 ``num_heads // num_kv_heads`` times smaller).
+
+Beyond the reference: ``rotary`` (queries and keys rotated to their positions, those of a
+``kv_cache`` counted) and prompts and decode steps over a ``PagedKVCache`` (``PagedSteps``).
 """
 
 from __future__ import annotations
@@ -23,10 +26,12 @@ import torch.nn as nn
 
 from ..ops.attention_forward import fastest_flash_attn_forward
 from ..ops.attention_func import fastest_flash_attn_func
-from ..utils import repeat_kv
+from ..utils import cached_tokens, repeat_kv
+from .flash_rotary import FastestFlashRotary
+from .paged import PagedSteps
 
 
-class FastestFlashGQA(nn.Module):
+class FastestFlashGQA(PagedSteps, nn.Module):
     def __init__(
         self,
         hidden_size: int,
@@ -38,6 +43,7 @@ class FastestFlashGQA(nn.Module):
         block_size: int = 0,
         softcap: Optional[float] = None,
         sliding_window: Optional[int] = None,
+        rotary: Optional[FastestFlashRotary] = None,
     ):
         super().__init__()
         self.hidden_size = hidden_size
@@ -48,12 +54,19 @@ class FastestFlashGQA(nn.Module):
         self.block_size = block_size
         self.softcap = softcap
         self.sliding_window = sliding_window
+        self.rotary = rotary
         assert num_heads % num_kv_heads == 0, "num_heads must be divisible by num_kv_heads"
         self.q_proj = nn.Linear(hidden_size, num_heads * self.head_dim, bias=bias)
         self.k_proj = nn.Linear(hidden_size, num_kv_heads * self.head_dim, bias=bias)
         self.v_proj = nn.Linear(hidden_size, num_kv_heads * self.head_dim, bias=bias)
         self.o_proj = nn.Linear(num_heads * self.head_dim, hidden_size, bias=bias)
         self.scale = 1.0 / math.sqrt(self.head_dim)
+
+    def _project(self, x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        B, S, _ = x.shape
+        return (self.q_proj(x).view(B, S, self.num_heads, self.head_dim).transpose(1, 2),
+                self.k_proj(x).view(B, S, self.num_kv_heads, self.head_dim).transpose(1, 2),
+                self.v_proj(x).view(B, S, self.num_kv_heads, self.head_dim).transpose(1, 2))
 
     def forward(
         self,
@@ -70,9 +83,9 @@ class FastestFlashGQA(nn.Module):
         B, S, _ = x.shape
         use_causal = self.default_causal if causal is None else causal
         bs = block_size or self.block_size or None
-        q = self.q_proj(x).view(B, S, self.num_heads, self.head_dim).transpose(1, 2)
-        k = self.k_proj(x).view(B, S, self.num_kv_heads, self.head_dim).transpose(1, 2)
-        v = self.v_proj(x).view(B, S, self.num_kv_heads, self.head_dim).transpose(1, 2)
+        q, k, v = self._project(x)
+        if self.rotary is not None:
+            q, k = self.rotary(q, k, q_offset=cached_tokens(kv_cache))
         if self.training and not return_lse and kv_cache is None:
             attn = fastest_flash_attn_func(
                 q, k, v, scale=self.scale, causal=use_causal, block_size=bs or 64,

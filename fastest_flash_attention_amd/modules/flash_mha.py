@@ -3,6 +3,9 @@
 Same constructor, weights, forward signature and outputs as the reference; the
 attention core is the HIP forward. q/k/v are passed as the strided
 ``[B, H, S, D]`` views of the projections (no copies: the kernel takes any strides).
+
+Beyond the reference: ``rotary`` (queries and keys rotated to their positions, those of a
+``kv_cache`` counted) and prompts and decode steps over a ``PagedKVCache`` (``PagedSteps``).
 """
 
 from __future__ import annotations
@@ -15,9 +18,12 @@ import torch.nn as nn
 
 from ..ops.attention_forward import fastest_flash_attn_forward
 from ..ops.attention_func import fastest_flash_attn_func
+from ..utils import cached_tokens
+from .flash_rotary import FastestFlashRotary
+from .paged import PagedSteps
 
 
-class FastestFlashMHA(nn.Module):
+class FastestFlashMHA(PagedSteps, nn.Module):
     def __init__(
         self,
         hidden_size: int,
@@ -29,6 +35,7 @@ class FastestFlashMHA(nn.Module):
         block_size: int = 0,
         softcap: Optional[float] = None,
         sliding_window: Optional[int] = None,
+        rotary: Optional[FastestFlashRotary] = None,
     ):
         super().__init__()
         self.hidden_size = hidden_size
@@ -41,6 +48,7 @@ class FastestFlashMHA(nn.Module):
         self.block_size = block_size
         self.softcap = softcap
         self.sliding_window = sliding_window
+        self.rotary = rotary
         self.q_proj = nn.Linear(hidden_size, hidden_size, bias=bias)
         self.k_proj = nn.Linear(hidden_size, hidden_size, bias=bias)
         self.v_proj = nn.Linear(hidden_size, hidden_size, bias=bias)
@@ -58,6 +66,11 @@ class FastestFlashMHA(nn.Module):
     def _heads(self, t: torch.Tensor, B: int, S: int) -> torch.Tensor:
         return t.view(B, S, self.num_heads, self.head_dim).transpose(1, 2)
 
+    def _project(self, x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        B, S, _ = x.shape
+        return (self._heads(self.q_proj(x), B, S), self._heads(self.k_proj(x), B, S),
+                self._heads(self.v_proj(x), B, S))
+
     def forward(
         self,
         x: torch.Tensor,
@@ -70,9 +83,9 @@ class FastestFlashMHA(nn.Module):
         B, S, _ = x.shape
         use_causal = self.default_causal if causal is None else causal
         bs = block_size or self.block_size or None
-        q = self._heads(self.q_proj(x), B, S)
-        k = self._heads(self.k_proj(x), B, S)
-        v = self._heads(self.v_proj(x), B, S)
+        q, k, v = self._project(x)
+        if self.rotary is not None:
+            q, k = self.rotary(q, k, q_offset=cached_tokens(kv_cache))
         if self.training and not return_lse and kv_cache is None:
             attn = fastest_flash_attn_func(
                 q, k, v, scale=self.scale, causal=use_causal, block_size=bs or 64,

@@ -34,6 +34,8 @@ import torch
 
 from ..kernels import _lib
 from .attention_forward import launch_prefill, prepare_prefill
+from .pages import PageBook, device_ints
+from .rotary import check_frequencies, check_magnitude
 
 
 def _auto_tokens_per_split(batch: int, heads_kv: int, max_len: int) -> int:
@@ -47,16 +49,6 @@ def _auto_tokens_per_split(batch: int, heads_kv: int, max_len: int) -> int:
     while tps > 64 and batch * heads_kv * max(1, -(-max_len // tps)) < 256:
         tps //= 2
     return tps
-
-
-def device_ints(values, device: torch.device) -> torch.Tensor:
-    """int32 tensor of ``values`` (a list or an int32 array) on ``device``. To a ROCm device
-    it goes through pinned memory, behind the work queued there, without waiting for it
-    (a captured stream keeps the waiting copy, which capture refuses)."""
-    t = torch.from_numpy(np.asarray(values, dtype=np.int32))
-    if device.type != "cuda" or t.numel() == 0 or torch.cuda.is_current_stream_capturing():
-        return t.to(device)
-    return t.pin_memory().to(device, non_blocking=True)
 
 
 def device_tables(tables: Sequence[Sequence[int]], lens: Sequence[int],
@@ -91,15 +83,19 @@ def set_append_pages(a: _lib.PagedAppendArgs, table: Sequence[int], start: int, 
 
 
 def check_page_ids(block_tables: torch.Tensor, context_lens: torch.Tensor, page_size: int,
-                   num_pages: int, max_context_len: int) -> None:
+                   num_pages: int, max_context_len: int,
+                   sliding_window: Optional[int] = None) -> None:
     """Raise IndexError if a page id the lengths reach lies outside ``[0, num_pages)``:
     entry j of row b is used when ``j * page_size < min(context_lens[b],
-    max_context_len)``. One device reduction and a host sync."""
+    max_context_len)`` and it holds a token of the window. One device reduction and a host
+    sync."""
     if block_tables.numel() == 0:
         return
     lens = torch.clamp(context_lens.to(torch.int64), min=0, max=max_context_len)
-    used = (torch.arange(block_tables.size(1), device=block_tables.device)[None, :] * page_size
-            < lens[:, None])
+    first = torch.arange(block_tables.size(1), device=block_tables.device)[None, :] * page_size
+    used = first < lens[:, None]
+    if sliding_window is not None:
+        used &= first + page_size > lens[:, None] - sliding_window
     bad = used & ((block_tables < 0) | (block_tables >= num_pages))
     if bool(bad.any()):
         b, j = (int(x) for x in bad.nonzero()[0])
@@ -120,7 +116,7 @@ def _paged_decode_fp32(q3, k_pages, v_pages, block_tables, context_lens, scale, 
     lens = [min(n, int(max_context_len))
             for n in context_lens.to(torch.int64).clamp(min=0).tolist()]
     bt = block_tables  # int32, contiguous, wide enough for max_context_len (checked)
-    check_page_ids(bt, context_lens, page_size, P_total, int(max_context_len))
+    check_page_ids(bt, context_lens, page_size, P_total, int(max_context_len), sliding_window)
     out = torch.zeros((B, Hq, D), dtype=torch.float32, device=q3.device)
     lse = (torch.full((B, Hq), float("-inf"), dtype=torch.float32, device=q3.device)
            if return_lse else None)
@@ -256,7 +252,8 @@ def fastest_flash_paged_decode(
     if q3.stride(-1) != 1 or q3.data_ptr() % 16 or q3.stride(0) % 8 or q3.stride(1) % 8:
         q3 = q3.contiguous() if not q3.is_contiguous() else q3.clone()
     if check_block_tables:
-        check_page_ids(block_tables, context_lens, page_size, P_total, max_context_len)
+        check_page_ids(block_tables, context_lens, page_size, P_total, max_context_len,
+                       sliding_window)
     if scale is None:
         scale = 1.0 / math.sqrt(D)
     if sliding_window is not None and int(sliding_window) <= 0:
@@ -306,6 +303,110 @@ def fastest_flash_paged_decode(
         if lse is not None:
             lse = lse[:, :, None, None]
     return out, lse
+
+
+def fastest_flash_paged_append(
+    k: torch.Tensor,
+    v: torch.Tensor,
+    k_pages: torch.Tensor,
+    v_pages: torch.Tensor,
+    block_tables: torch.Tensor,
+    positions: torch.Tensor,
+    *,
+    q: Optional[torch.Tensor] = None,
+    inv_freq: Optional[torch.Tensor] = None,
+    interleaved: bool = False,
+    magnitude: float = 1.0,
+    counts: Optional[torch.Tensor] = None,
+) -> Optional[torch.Tensor]:
+    """Write the new tokens of a batch of sequences into the page pools, in one launch; with
+    ``inv_freq`` their keys are rotated on the way (``fastest_flash_rotary``), and their
+    queries ``q`` too, which are returned as a new tensor (None without ``q``).
+
+    k, v: ``[B, Hkv, n, D]`` or, one token per sequence, ``[B, Hkv, D]``; q alike with its own
+    heads; pools ``[P, Hkv, page_size, D]``; block_tables int32 ``[B, max_blocks]``; positions
+    int32 ``[B]``. Token j of sequence b is token ``positions[b] + j`` of the sequence: page
+    ``block_tables[b, t // page_size]``, slot ``t % page_size``, rotated by position t. The
+    pages have to be the sequence's own. A token is left out (its query is rotated all the
+    same) where ``positions[b] + j`` is negative or past the table, its page id lies outside
+    the pool, or ``j >= counts[b]`` (int32 ``[B]``, batches of unequal lengths). Everything is
+    read from the device, so the call can be captured into a graph. No gradients.
+    """
+    one = k.dim() == 3
+    if one:
+        k, v = k.unsqueeze(2), v.unsqueeze(2) if v.dim() == 3 else v
+        q = q.unsqueeze(2) if q is not None and q.dim() == 3 else q
+    if k.dim() != 4 or k.shape != v.shape:
+        raise ValueError("k and v must both be [B, Hkv, n, D] or [B, Hkv, D]")
+    B, Hkv, n, D = k.shape
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
+        raise ValueError("k_pages / v_pages must both be [num_pages, Hkv, page_size, D]")
+    if k_pages.size(1) != Hkv or k_pages.size(3) != D:
+        raise ValueError(f"k {tuple(k.shape)} does not match the pools {tuple(k_pages.shape)}")
+    if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
+        raise ValueError("page pools must be contiguous")
+    if not (k.dtype == v.dtype == k_pages.dtype == v_pages.dtype) or (q is not None and q.dtype != k.dtype):
+        raise TypeError("q, k, v and the page pools must share a dtype")
+    code = _lib.dtype_code(k.dtype, allow_fp32=True)
+    if q is not None:
+        if inv_freq is None:
+            raise ValueError("q is rotated only: it needs inv_freq")
+        if q.dim() != 4 or (q.size(0), q.size(2), q.size(3)) != (B, n, D):
+            raise ValueError(f"q {tuple(q.shape)} does not match k {tuple(k.shape)}")
+    if block_tables.dim() != 2 or block_tables.size(0) != B:
+        raise ValueError(f"block_tables must be [B, max_blocks] with B {B}")
+    for name, t in (("positions", positions), ("counts", counts)):
+        if t is not None and tuple(t.shape) != (B,):
+            raise ValueError(f"{name} must be [B] with B {B}")
+    if block_tables.dtype != torch.int32 or positions.dtype != torch.int32 or (
+            counts is not None and counts.dtype != torch.int32):
+        raise TypeError("block_tables, positions and counts must be int32")
+    device = k.device
+    for name, t in (("k", k), ("v", v), ("q", q), ("k_pages", k_pages), ("v_pages", v_pages),
+                    ("block_tables", block_tables), ("positions", positions), ("counts", counts)):
+        if t is None:
+            continue
+        if t.device.type != "cuda":
+            raise RuntimeError("fastest_flash_attention_amd paged append runs on ROCm tensors only; "
+                               f"{name} is on {t.device}")
+        if t.device != device:
+            raise RuntimeError(f"{name} is on {t.device}, k on {device}")
+    a = _lib.PagedAppendBatchArgs()
+    if inv_freq is not None:
+        inv_freq = check_frequencies(inv_freq, D, device)
+        a.inv_freq = inv_freq.data_ptr()
+        a.rotary_dim = 2 * inv_freq.numel()
+    a.magnitude = check_magnitude(magnitude)
+    a.interleaved = 1 if interleaved else 0
+    k, v = (t if D == 1 or t.stride(3) == 1 else t.contiguous() for t in (k, v))
+    out = None
+    if q is not None:
+        q = q if D == 1 or q.stride(3) == 1 else q.contiguous()
+        out = torch.empty_like(q)
+        if D > 1 and out.stride(3) != 1:
+            out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        a.q, a.q_out, a.heads_q = q.data_ptr(), out.data_ptr(), q.size(1)
+        a.q_stride[:] = list(q.stride()[:3])
+        a.q_out_stride[:] = list(out.stride()[:3])
+    block_tables, positions = block_tables.contiguous(), positions.contiguous()
+    counts = counts.contiguous() if counts is not None else None
+    a.k_pages, a.v_pages = k_pages.data_ptr(), v_pages.data_ptr()
+    a.k_new, a.v_new = k.data_ptr(), v.data_ptr()
+    a.k_new_stride[:] = list(k.stride()[:3])
+    a.v_new_stride[:] = list(v.stride()[:3])
+    a.block_tables, a.positions = block_tables.data_ptr(), positions.data_ptr()
+    a.counts = counts.data_ptr() if counts is not None else None
+    a.block_table_stride = block_tables.size(1)
+    a.batch, a.heads_kv, a.n_tokens, a.head_dim = B, Hkv, n, D
+    a.page_size, a.num_pages = k_pages.size(2), k_pages.size(0)
+    a.dtype = code
+    if block_tables.numel() and k_pages.numel():
+        _lib.launch(_lib.load().ffa_paged_append_batch, a, device)
+    elif out is not None and out.numel():
+        raise ValueError("the page pools or block_tables are empty")
+    if out is not None and one:
+        out = out.squeeze(2)
+    return out
 
 
 class ContinuousKVCache:
@@ -375,8 +476,12 @@ class ContinuousKVCache:
         return self.k_cache[:batch_size, :, :max_len, :], self.v_cache[:batch_size, :, :max_len, :]
 
 
-class PagedKVCache:
+class PagedKVCache(PageBook):
     """Paged KV-cache (vLLM-style page tables), reference ops/kv_cache.py:110-240.
+
+    Beyond the reference: batched decode and append, sequences that share pages
+    (``fork_sequence``, copy on write), ``truncate_sequence``, ``evict`` (pages that a sliding
+    window has left behind) and ``compact``.
 
     Args:
         max_pages: total number of physical pages.
@@ -406,6 +511,10 @@ class PagedKVCache:
                                    dtype=dtype, device=device)
         self.free_pages = list(range(max_pages))
         self.sequences: dict = {}
+        self._init_pages()
+
+    def _pools(self):
+        return self.k_pages, self.v_pages
 
     def allocate_page(self) -> int:
         """Take the first free physical page (reference :157-161)."""
@@ -414,10 +523,11 @@ class PagedKVCache:
         return self.free_pages.pop(0)
 
     def free_sequence(self, seq_id: int):
-        """Return a sequence's pages to the tail of the free list (reference :163-168)."""
+        """Return a sequence's pages to the tail of the free list (reference :163-168); pages
+        of a forked sequence stay with their other owners."""
         if seq_id in self.sequences:
             for page_id in self.sequences[seq_id]["page_table"]:
-                self.free_pages.append(page_id)
+                self._release(page_id)
             del self.sequences[seq_id]
 
     def append_tokens(self, seq_id: int, k_tokens: torch.Tensor, v_tokens: torch.Tensor) -> int:
@@ -435,6 +545,10 @@ class PagedKVCache:
             return seq["len"]
         L0 = seq["len"]
         P = self.page_size
+        if self._owners:
+            if self._pages_to_own([seq]) > len(self.free_pages):
+                raise RuntimeError("PagedKVCache: out of physical pages")
+            self._own_last_pages([seq])
         need_pages = (L0 + S_new + P - 1) // P
         out_of_pages = False
         while len(seq["page_table"]) < need_pages:
@@ -460,6 +574,87 @@ class PagedKVCache:
         if out_of_pages:
             raise RuntimeError("PagedKVCache: out of physical pages")
         return seq["len"]
+
+    def append_batch(
+        self,
+        seq_ids: Sequence[int],
+        k: torch.Tensor,
+        v: torch.Tensor,
+        *,
+        q: Optional[torch.Tensor] = None,
+        rotary=None,
+    ) -> Optional[torch.Tensor]:
+        """Append ``[B, num_heads, n, head_dim]`` (or ``[B, num_heads, head_dim]``) K/V, row b to
+        sequence ``seq_ids[b]``, in one launch. With ``rotary`` (a ``FastestFlashRotary``) the
+        keys, and the queries ``q`` of the same tokens, are rotated to the tokens' positions on
+        the way; the rotated queries are returned. Sequences are created as needed, and may not
+        repeat. When the pool has too few free pages nothing is appended (RuntimeError)."""
+        n = 1 if k.dim() == 3 else k.size(2)
+        if len(seq_ids) != k.size(0):
+            raise ValueError(f"{len(seq_ids)} sequences for a batch of {k.size(0)}")
+        if len(set(seq_ids)) != len(seq_ids):
+            raise ValueError("a sequence appears twice")
+        if k.shape != v.shape or k.size(1) != self.num_heads or k.size(-1) != self.head_dim:
+            raise ValueError(f"k {tuple(k.shape)} / v {tuple(v.shape)} do not match the cache")
+        if q is not None and rotary is None:
+            raise ValueError("q is rotated only: it needs rotary")
+        device, P = self.k_pages.device, self.page_size
+        if rotary is not None and device.type != "cuda":
+            raise RuntimeError(f"the rotation runs on ROCm tensors only; the pools are on {device}")
+        known = [self.sequences.get(s) or {"page_table": [], "len": 0} for s in seq_ids]
+        need = self._pages_to_own(known) if n and self._owners else 0
+        need += sum(max(0, -(-(s["len"] + n) // P) - len(s["page_table"])) for s in known)
+        if need > len(self.free_pages):
+            raise RuntimeError("PagedKVCache: out of physical pages")
+        if n == 0:
+            return q
+        if device.type != "cuda":
+            for i, s in enumerate(seq_ids):
+                self.append_tokens(s, k[i].reshape(self.num_heads, n, -1), v[i].reshape(self.num_heads, n, -1))
+            return None
+        dt = self.k_pages.dtype
+        k, v = k.to(device, dt), v.to(device, dt)
+        if self._owners:
+            self._own_last_pages(known)
+        for seq_id, seq in zip(seq_ids, known):
+            self.sequences[seq_id] = seq
+            while len(seq["page_table"]) * P < seq["len"] + n:
+                seq["page_table"].append(self.allocate_page())
+        tables, at = device_tables([s["page_table"] for s in known], [s["len"] for s in known], device)
+        out = fastest_flash_paged_append(
+            k, v, self.k_pages, self.v_pages, tables, at, q=q,
+            **(rotary.append_options(device) if rotary is not None else {}))
+        for seq in known:
+            seq["len"] += n
+        return out
+
+    def evict(self, seq_id: int, sliding_window: int, sink_tokens: int = 0) -> int:
+        """Release the pages of a sequence that hold none of its last ``sliding_window`` tokens
+        and none of its first ``sink_tokens``: attention over that window (or a smaller one)
+        with those sinks (or fewer) no longer reads them. Returns how many were released.
+        ``decode`` with a larger window and ``get_kv`` refuse the sequence afterwards."""
+        if sliding_window <= 0 or sink_tokens < 0:
+            raise ValueError("sliding_window must be positive and sink_tokens not negative")
+        seq = self._sequence(seq_id)
+        table, P = seq["page_table"], self.page_size
+        gone = 0
+        for j in range(-(-sink_tokens // P), max(0, seq["len"] - sliding_window) // P):
+            if table[j] >= 0:
+                self._release(table[j])
+                table[j] = -1
+                gone += 1
+        return gone
+
+    def _check_seen(self, seq_ids, sliding_window, sink_tokens) -> None:
+        """ValueError if a sequence lacks a page that attention from its last token reads."""
+        for s in seq_ids:
+            seq = self.sequences.get(s)
+            if seq is None or -1 not in seq["page_table"]:
+                continue
+            table, P = seq["page_table"], self.page_size
+            low = max(0, seq["len"] - sliding_window) if sliding_window else 0
+            if -1 in table[low // P:] or -1 in table[:-(-min(sink_tokens, low) // P)]:
+                raise ValueError(f"sequence {s} has evicted pages within the attention's window or sinks")
 
     def _append_device(self, seq: dict, start: int, kn: torch.Tensor, vn: torch.Tensor) -> None:
         """One ``ffa_paged_append`` launch: scatter [H, n, D] new rows into the pages."""
@@ -512,6 +707,8 @@ class PagedKVCache:
         launch; a host pool by one indexed host copy."""
         if seq_id not in self.sequences or self.sequences[seq_id]["len"] == 0:
             return None, None
+        if -1 in self.sequences[seq_id]["page_table"]:
+            raise ValueError(f"sequence {seq_id} has evicted pages")
         if self.k_pages.device.type != "cuda":
             return self._get_kv_host(seq_id)
         if self.k_pages.element_size() not in (2, 4):
@@ -562,6 +759,7 @@ class PagedKVCache:
     ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
         """Decode attention of ``q`` (``[B, Hq, D]``, one token per sequence of
         ``seq_ids``) over the cached tokens, read in place from the pages."""
+        self._check_seen(seq_ids, sliding_window, 0)
         bt, lens = self.block_tables(seq_ids)
         max_len = max([0] + [self.sequences[s]["len"] for s in seq_ids if s in self.sequences])
         return fastest_flash_paged_decode(

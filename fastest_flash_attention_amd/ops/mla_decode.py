@@ -26,6 +26,7 @@ import torch
 
 from ..kernels import _lib
 from .kv_cache import check_page_ids, device_tables, set_append_pages
+from .pages import PageBook
 
 MLA_ROPE_DIM = 64
 MLA_LATENT_DIMS = (256, 512)
@@ -268,14 +269,15 @@ def mla_assemble(q_nope: torch.Tensor, q_rope: torch.Tensor, kv: torch.Tensor,
     return q, k
 
 
-class MLALatentCache:
+class MLALatentCache(PageBook):
     """Paged cache of MLA latent rows ``[c_t | r_t]`` (latent_dim + rope_dim values per
     token, shared by all heads).
 
     Page bookkeeping follows PagedKVCache (reference ops/kv_cache.py:110-240): a free
     list popped from the front, per-sequence page tables, token t of a sequence at
     ``(page_table[t // page_size], t % page_size)``, pages returned to the tail of the
-    free list. ``pages`` is ``[max_pages, page_size, latent_dim + rope_dim]``.
+    free list. ``pages`` is ``[max_pages, page_size, latent_dim + rope_dim]``. Sequences may
+    share pages (``fork_sequence``, ``truncate_sequence``, ``compact``).
     """
 
     def __init__(self, max_pages: int = 1024, page_size: int = 64, latent_dim: int = 512,
@@ -289,6 +291,10 @@ class MLALatentCache:
                                  device=device)
         self.free_pages = list(range(max_pages))
         self.sequences: dict = {}
+        self._init_pages()
+
+    def _pools(self):
+        return self.pages, None
 
     def allocate_page(self) -> int:
         if not self.free_pages:
@@ -297,7 +303,8 @@ class MLALatentCache:
 
     def free_sequence(self, seq_id: int) -> None:
         if seq_id in self.sequences:
-            self.free_pages.extend(self.sequences[seq_id]["page_table"])
+            for page_id in self.sequences[seq_id]["page_table"]:
+                self._release(page_id)
             del self.sequences[seq_id]
 
     def seq_len(self, seq_id: int) -> int:
@@ -316,6 +323,10 @@ class MLALatentCache:
         if S_new == 0:
             return seq["len"]
         L0, P = seq["len"], self.page_size
+        if self._owners:
+            if self._pages_to_own([seq]) > len(self.free_pages):
+                raise RuntimeError("MLALatentCache: out of physical pages")
+            self._own_last_pages([seq])
         need_pages = (L0 + S_new + P - 1) // P
         out_of_pages = False
         while len(seq["page_table"]) < need_pages:

@@ -55,6 +55,11 @@ def maybe_unsqueeze_head(
     return q, k, v, False
 
 
+def cached_tokens(kv_cache) -> int:
+    """Tokens that a module's ``kv_cache`` (``(K, V)`` or None) holds."""
+    return 0 if kv_cache is None else kv_cache[0].size(-2)
+
+
 def repeat_kv(kv: torch.Tensor, num_q_heads: int, num_kv_heads: int) -> torch.Tensor:
     """Materialise GQA/MQA KV heads: q head h uses kv head h // (Hq // Hkv)
     (reference utils.py:111-130). The HIP kernels apply this map by index instead."""

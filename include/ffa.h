@@ -35,6 +35,9 @@
  *   ffa_rope_tables        <- RotaryEmbedding's cos and sin (modules/flash_mla.py:42-48).
  *   ffa_mla_assemble       <- q and k of FastestFlashMLA.forward (modules/flash_mla.py:
  *                             129-152): RoPE of the rope parts and the concatenations.
+ *   ffa_rotary, ffa_paged_append_batch, ffa_paged_copy: no counterpart; rotary positions
+ *                             for any model's queries and keys, a batch's new tokens into
+ *                             the paged pool in one launch, page copies (forks, compaction).
  *   ffa_attn_bwd           <- fastest_flash_attn_backward   ops/attention_backward.py:19-76
  *                             (its GPU branch flash_attn_triton_backward
  *                              kernels/triton_bwd.py:122-190; the CPU branch
@@ -55,7 +58,7 @@
 extern "C" {
 #endif
 
-#define FFA_ABI_VERSION 13
+#define FFA_ABI_VERSION 14
 
 typedef enum ffa_status {
   FFA_OK = 0,
@@ -450,6 +453,107 @@ typedef struct ffa_mla_assemble_args {
 } ffa_mla_assemble_args;
 
 int ffa_mla_assemble(const ffa_mla_assemble_args* args, void* stream);
+
+/*
+ * Rotary positions of queries and keys. Pair i < rotary_dim / 2 of the row at position t
+ * turns by the angle t * inv_freq[i] (formed in 64 bits):
+ *   (a, b) -> magnitude * (a cos - b sin, b cos + a sin)
+ * a, b = dims i and i + rotary_dim / 2, or 2i and 2i + 1 with interleaved; dims from
+ * rotary_dim on pass through unchanged. inverse turns by the opposite angle: the gradient.
+ *   q, q_out : [batch, heads_q, seqlen, head_dim], k, k_out with heads_k: element strides
+ *              [batch, head, token], dim stride 1; a count of 0 heads leaves a tensor out.
+ *              Outputs do not overlap inputs and have no broadcast strides. Any strides and
+ *              element-aligned addresses; 16-byte aligned rows are fastest.
+ *   positions: NULL: q_offset + token. Else device integers of position_bytes (4 or 8) with
+ *              element strides [batch, token].
+ * Products and sums are fp32, rounded once to dtype.
+ */
+typedef struct ffa_rotary_args {
+  const void* q;
+  const void* k;
+  void* q_out;
+  void* k_out;
+  const double* inv_freq;   /* device, [rotary_dim / 2] */
+  const void* positions;
+  int64_t q_stride[3];
+  int64_t k_stride[3];
+  int64_t q_out_stride[3];
+  int64_t k_out_stride[3];
+  int64_t position_stride[2];
+  int64_t q_offset;
+  int32_t batch;
+  int32_t heads_q;
+  int32_t heads_k;
+  int32_t seqlen;
+  int32_t head_dim;
+  int32_t rotary_dim;       /* even, 2 .. head_dim */
+  int32_t position_bytes;
+  int32_t interleaved;
+  int32_t inverse;
+  float magnitude;          /* finite */
+  int32_t dtype;            /* ffa_dtype */
+} ffa_rotary_args;
+
+int ffa_rotary(const ffa_rotary_args* args, void* stream);
+
+/*
+ * The new tokens of a batch of sequences into the paged pools, in one launch: token j of
+ * sequence b is token positions[b] + j of that sequence and goes to its page
+ * block_tables[b][(positions[b] + j) / page_size], slot (positions[b] + j) % page_size. With
+ * rotary_dim > 0 the keys are rotated on the way as in ffa_rotary, and the tokens' queries
+ * (heads_q > 0) into q_out; values are copied. A token is left out (nothing of the pools is
+ * written) where its position is negative, j >= counts[b], its page lies past the table's
+ * row or its page id outside [0, num_pages). Two tokens must not share a slot.
+ *   q, q_out : [batch, heads_q, n_tokens, head_dim], k_new, v_new with heads_kv: element
+ *              strides [batch, head, token], dim stride 1.
+ */
+typedef struct ffa_paged_append_batch_args {
+  void* k_pages;
+  void* v_pages;
+  const void* k_new;
+  const void* v_new;
+  const void* q;
+  void* q_out;
+  const double* inv_freq;        /* device, [rotary_dim / 2] */
+  const int32_t* block_tables;   /* [batch, block_table_stride] */
+  const int32_t* positions;      /* [batch] */
+  const int32_t* counts;         /* [batch], or NULL: n_tokens each */
+  int64_t k_new_stride[3];
+  int64_t v_new_stride[3];
+  int64_t q_stride[3];
+  int64_t q_out_stride[3];
+  int32_t block_table_stride;
+  int32_t batch;
+  int32_t heads_q;               /* 0: no queries */
+  int32_t heads_kv;
+  int32_t n_tokens;
+  int32_t head_dim;
+  int32_t rotary_dim;            /* 0: no rotation */
+  int32_t page_size;
+  int32_t num_pages;
+  int32_t interleaved;
+  float magnitude;
+  int32_t dtype;                 /* ffa_dtype, of the pools too */
+} ffa_paged_append_batch_args;
+
+int ffa_paged_append_batch(const ffa_paged_append_batch_args* args, void* stream);
+
+/*
+ * Page src[i] of the pools onto page dst[i], i < n_pairs. The destinations must be distinct
+ * and none of them a source (the copies run in any order). A pair with an id outside
+ * [0, num_pages) is left out. v_pages may be NULL (one pool).
+ */
+typedef struct ffa_paged_copy_args {
+  void* k_pages;
+  void* v_pages;
+  const int32_t* src;      /* device, [n_pairs] */
+  const int32_t* dst;
+  int64_t page_bytes;      /* of one page of one pool, a multiple of 2 */
+  int32_t n_pairs;
+  int32_t num_pages;
+} ffa_paged_copy_args;
+
+int ffa_paged_copy(const ffa_paged_copy_args* args, void* stream);
 
 /*
  * Attention backward (recompute): gradients of the prefill forward above for one
