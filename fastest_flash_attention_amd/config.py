@@ -1,8 +1,9 @@
 """Attention configuration — the same dataclass as the reference (config.py:14-81).
 
 Fields read on the forward path: causal, sliding_window, softcap, num_kv_heads,
-compute_dtype, two_pass, return_lse, block_size_q/kv. When a config is passed to
-``fastest_flash_attn_forward`` its causal/softcap/sliding_window/two_pass/
+compute_dtype, two_pass, return_lse, block_size_q/kv and, beyond the reference, sink_tokens
+(first keys that a sliding window leaves visible). When a config is passed to
+``fastest_flash_attn_forward`` its causal/softcap/sliding_window/sink_tokens/two_pass/
 compute_dtype/num_kv_heads/return_lse override the keyword arguments, and its block
 sizes apply only when ``block_size`` is None (reference ops/attention_forward.py:66-73,
 102-105). use_triton, pipeline_stages, dropout_p, deterministic, max_seqlen_q/kv and
@@ -35,6 +36,7 @@ class AttentionConfig:
     max_seqlen_q: int = 0
     max_seqlen_kv: int = 0
     page_size: int = 64
+    sink_tokens: int = 0
 
     def resolve_block_sizes(self, S_q: int, S_kv: int, D: int) -> Tuple[int, int]:
         """(block_q, block_kv); a zero field is auto-selected (reference config.py:75-81)."""

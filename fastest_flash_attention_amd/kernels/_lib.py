@@ -20,7 +20,7 @@ import torch  # noqa: F401  (must load torch's HIP runtime before libffa.so)
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libffa.so")
 
-FFA_ABI_VERSION = 14
+FFA_ABI_VERSION = 15
 FFA_DTYPE_BF16 = 0
 FFA_DTYPE_FP16 = 1
 FFA_DTYPE_FP32 = 2
@@ -74,6 +74,7 @@ class PrefillArgs(ctypes.Structure):
         ("cache_len", ctypes.c_int32),
         ("workspace", ctypes.c_void_p),
         ("workspace_bytes", ctypes.c_size_t),
+        ("sinks", ctypes.c_int32),
     ]
 
 
@@ -166,6 +167,7 @@ class PagedDecodeArgs(ctypes.Structure):
         ("scale", ctypes.c_float),
         ("softcap", ctypes.c_float),
         ("dtype", ctypes.c_int32),
+        ("sinks", ctypes.c_int32),
     ]
 
 
@@ -352,6 +354,7 @@ class AttnBwdArgs(ctypes.Structure):
         ("softcap", ctypes.c_float),
         ("dtype", ctypes.c_int32),
         ("v_head_dim", ctypes.c_int32),
+        ("sinks", ctypes.c_int32),
     ]
 
 

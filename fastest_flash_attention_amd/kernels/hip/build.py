@@ -22,8 +22,9 @@ PKG_KERNELS = os.path.dirname(HERE)
 REPO = os.path.dirname(os.path.dirname(PKG_KERNELS))
 INCLUDE = os.path.join(REPO, "include")
 OUT_LIB = os.path.join(PKG_KERNELS, "libffa.so")
-SOURCES = ["ffa_api.hip", "ffa_prefill.hip", "ffa_decode.hip", "ffa_backward.hip", "ffa_mla.hip",
-           "ffa_mask.hip", "ffa_rotary.hip", "ffa_pages.hip"]
+SOURCES = ["ffa_api.hip", "ffa_prefill.hip", "ffa_prefill_sinks.hip", "ffa_decode.hip",
+           "ffa_backward.hip", "ffa_backward_sinks.hip", "ffa_mla.hip", "ffa_mask.hip",
+           "ffa_rotary.hip", "ffa_pages.hip"]
 ARCH = "gfx950"
 
 # -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 are emitted (scalar fp32 VALU only).

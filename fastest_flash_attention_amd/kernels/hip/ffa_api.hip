@@ -26,6 +26,13 @@ int check_v_head_dim(int32_t v_head_dim, int32_t head_dim, int32_t dtype) {
   return v_head_dim % 8 != 0 ? FFA_ERR_MISALIGNED : FFA_OK;
 }
 
+// sinks: not negative, and (where they count) not with a narrower V.
+int check_sinks(int32_t sinks, int32_t window, int32_t v_head_dim, int32_t head_dim) {
+  if (sinks < 0) return FFA_ERR_INVALID_ARG;
+  if (sinks > 0 && window > 0 && v_head_dim != 0 && v_head_dim != head_dim) return FFA_ERR_UNSUPPORTED_HEAD_DIM;
+  return FFA_OK;
+}
+
 // rotary_dim: even, within the head. magnitude: finite.
 bool valid_rotary(int32_t rotary_dim, int32_t head_dim, float magnitude) {
   return rotary_dim >= 0 && rotary_dim % 2 == 0 && rotary_dim <= head_dim && std::isfinite(magnitude);
@@ -43,7 +50,7 @@ int check_decode_args(const ffa_paged_decode_args* a, bool* empty) {
   if (!valid_dtype(a->dtype)) return FFA_ERR_UNSUPPORTED_DTYPE;
   if (a->head_dim < 1 || a->head_dim > 256) return FFA_ERR_UNSUPPORTED_HEAD_DIM;
   if (a->batch < 0 || a->heads_q < 1 || a->heads_kv < 1 || a->page_size < 1 ||
-      a->num_pages < 0 || a->max_context_len < 0 || a->tokens_per_split < 0) {
+      a->num_pages < 0 || a->max_context_len < 0 || a->tokens_per_split < 0 || a->sinks < 0) {
     return FFA_ERR_INVALID_ARG;
   }
   if (a->heads_q % a->heads_kv != 0) return FFA_ERR_GQA_RATIO;
@@ -89,6 +96,8 @@ int check_prefill_args(const ffa_prefill_args* a, bool* empty) {
   if (a->batch < 0 || a->heads_q < 1 || a->heads_kv < 1 || a->seqlen_q < 0 || a->seqlen_kv < 0) {
     return FFA_ERR_INVALID_ARG;
   }
+  if (const int rc = check_sinks(a->sinks, a->window, a->v_head_dim, a->head_dim); rc != FFA_OK) return rc;
+  if (a->sinks > 0 && a->window > 0 && a->block_key_mask != nullptr) return FFA_ERR_INVALID_ARG;
   if (a->heads_q % a->heads_kv != 0) return FFA_ERR_GQA_RATIO;
   const bool cached = a->k_cache != nullptr;
   if (cached && (a->cache_len < 0 || a->cache_len > a->seqlen_kv || a->v_cache == nullptr)) {
@@ -208,7 +217,7 @@ int ffa_prefill_fwd(const ffa_prefill_args* a, void* stream) {
 size_t ffa_prefill_workspace_bytes(const ffa_prefill_args* a) {
   if (a == nullptr || a->batch < 0 || a->heads_q < 1 || a->heads_kv < 1 ||
       a->heads_q % a->heads_kv != 0 || a->seqlen_q < 0 || a->seqlen_kv < 0 || a->head_dim < 1 ||
-      a->head_dim > 256 || (a->k_cache != nullptr && (a->cache_len < 0 || a->cache_len > a->seqlen_kv))) {
+      a->head_dim > 256 || a->sinks < 0 || (a->k_cache != nullptr && (a->cache_len < 0 || a->cache_len > a->seqlen_kv))) {
     return 0;
   }
   return ffa::prefill_workspace_bytes(*a);
@@ -291,7 +300,7 @@ int ffa_paged_decode_fwd(const ffa_paged_decode_args* a, void* stream) {
   const int rc = check_decode_args(a, &empty);
   if (rc != FFA_OK || empty) return rc;
   const size_t need = ffa::decode_workspace_bytes(a->batch, a->heads_q, a->head_dim,
-                                                  a->max_context_len, a->tokens_per_split);
+                                                  ffa::decode_span(*a), a->tokens_per_split);
   if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need)) return FFA_ERR_WORKSPACE;
   if ((reinterpret_cast<uintptr_t>(a->workspace) & 15u) != 0) return FFA_ERR_MISALIGNED;
   return ffa::launch_paged_decode(*a, static_cast<hipStream_t>(stream));
@@ -476,7 +485,7 @@ size_t ffa_attn_bwd_split_workspace_bytes(const ffa_attn_bwd_args* a) {
       a->heads_q % a->heads_kv != 0 || a->seqlen_q < 0 || a->seqlen_kv < 0 || a->head_dim < 1 ||
       a->head_dim > 256 || a->v_head_dim < 0 || a->v_head_dim > a->head_dim ||
       a->seqlen_q > ffa::kMaxPos || a->seqlen_kv > ffa::kMaxPos || a->q_offset > ffa::kMaxPos ||
-      a->q_offset < -ffa::kMaxPos) {
+      a->q_offset < -ffa::kMaxPos || a->sinks < 0) {
     return 0;
   }
   return ffa::attn_bwd_split_workspace_bytes(*a);
@@ -490,6 +499,7 @@ int ffa_attn_bwd(const ffa_attn_bwd_args* a, void* stream) {
   if (a->batch < 0 || a->heads_q < 1 || a->heads_kv < 1 || a->seqlen_q < 0 || a->seqlen_kv < 0) {
     return FFA_ERR_INVALID_ARG;
   }
+  if (const int rc = check_sinks(a->sinks, a->window, a->v_head_dim, a->head_dim); rc != FFA_OK) return rc;
   if (a->heads_q % a->heads_kv != 0) return FFA_ERR_GQA_RATIO;
   if (a->batch == 0 || a->seqlen_q == 0) return FFA_OK;
   if (a->dout == nullptr || a->q == nullptr || a->o == nullptr || a->lse == nullptr ||

@@ -85,6 +85,23 @@ struct Elem<F16Tag> {
   }
 };
 
+// Marks the element tag of a kernel compiled for a sliding window with sinks: the first
+// `sinks` keys stay visible behind the window. Kernels of calls without sinks hold none of
+// their code.
+template <typename Tag>
+struct Sinks {};
+template <typename Tag>
+struct Elem<Sinks<Tag>> : Elem<Tag> {};
+template <typename Tag>
+constexpr bool kSinks = false;
+template <typename Tag>
+constexpr bool kSinks<Sinks<Tag>> = true;
+// the tag without the mark
+template <typename Tag>
+struct Unsunk { using type = Tag; };
+template <typename Tag>
+struct Unsunk<Sinks<Tag>> { using type = Tag; };
+
 __device__ inline float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ inline float fast_log2(float x) { return __builtin_amdgcn_logf(x); }
 
@@ -164,6 +181,13 @@ __host__ __device__ inline int clamp_window(int window, int q_offset, int seqlen
   if (window <= 0) return 0;
   const int64_t lim = static_cast<int64_t>(q_offset) + seqlen_q + 1;
   return static_cast<int>(window < lim ? window : (lim < 1 ? 1 : lim));
+}
+
+// The sinks that a call's kernels have to know of: 0 without a window, and where every row's
+// window reaches key 0.
+__host__ __device__ inline int clamp_sinks(int sinks, int window, int q_offset, int seqlen_q) {
+  if (window <= 0 || sinks <= 0 || static_cast<int64_t>(q_offset) + seqlen_q <= window) return 0;
+  return sinks < kMaxPos ? sinks : kMaxPos;
 }
 
 // Eight consecutive 16-bit elements row[d0 .. d0+7] as one 128-bit value, zero

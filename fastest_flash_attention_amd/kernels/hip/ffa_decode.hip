@@ -69,6 +69,7 @@ struct DecodeParams {
   int bt_stride;
   int B, Hq, Hkv, G, D, P, log2P, num_pages;
   int n_splits, tps, window;
+  int sinks;    // first tokens seen besides the window (0: none)
   int max_len;  // context lengths are clamped to this (it sizes the grid)
   int n_cg;
   int dp;
@@ -112,6 +113,11 @@ __device__ inline int dec_kswz(int r) {
   return r & 15;
 }
 
+// Sinks (Tag = Sinks<...>): the tokens seen, the first `ns` and then the window from `lo` on,
+// are numbered one after another, and splits and tiles cut that numbering, so a sequence takes
+// as many workgroups as it has tokens to read, however long it is; only the page lookups and
+// nothing of the arithmetic knows of the gap. On MI355X (B 64, 32/8 heads, D 128, 16-token
+// pages, L~U[512, 32768], window 4096, 4 sinks): SINKFIGURE.
 template <typename Tag, int DP, bool SOFTCAP>
 __global__ __launch_bounds__(kDecThreads, kDecMinBlocks<DP>) void decode_split_kernel(
     const DecodeParams p) {
@@ -144,8 +150,11 @@ __global__ __launch_bounds__(kDecThreads, kDecMinBlocks<DP>) void decode_split_k
   const int cg = hkcg - hk * p.n_cg;
   const int L = min(max(p.lens[b], 0), p.max_len);
   const int lo = p.window > 0 ? max(0, L - p.window) : 0;
-  const int s_begin = max(split * p.tps, lo);
-  const int s_end = min(split * p.tps + p.tps, L);
+  constexpr bool SINK = kSinks<Tag>;
+  const int ns = SINK ? min(p.sinks, lo) : 0;  // sinks outside the window
+  const int gap = lo - ns;                     // token number - position in the numbering, past them
+  const int s_begin = SINK ? split * p.tps : max(split * p.tps, lo);
+  const int s_end = min(split * p.tps + p.tps, SINK ? L - gap : L);
   if (s_begin >= s_end) return;  // uniform across the workgroup: no barrier reached
 
   const int tid = threadIdx.x;
@@ -159,17 +168,32 @@ __global__ __launch_bounds__(kDecThreads, kDecMinBlocks<DP>) void decode_split_k
   const int dchunks = D >> 3;
 
   // Stage the split's physical page ids (entries [pg0, pg1]) in LDS.
+  // (with sinks: those of the split's sinks first, n_sp of them)
   int slot0;
-  const int pg0 = page_of(p, s_begin, slot0);
+  const int pg0 = page_of(p, SINK && s_end > ns ? max(s_begin, ns) + gap : s_begin, slot0);
   int slot1;
-  const int pg1 = page_of(p, s_end - 1, slot1);
+  const int pg1 = SINK && s_end <= ns ? pg0 - 1 : page_of(p, s_end - 1 + gap * SINK, slot1);
+  int sp0 = 0, n_sp = 0;
+  if (SINK && s_begin < ns) {
+    sp0 = page_of(p, s_begin, slot0);
+    n_sp = page_of(p, min(s_end, ns) - 1, slot1) - sp0 + 1;
+  }
+  // entry of bt_lds, and slot in the page, of position `e` of the numbering
+  auto locate = [&](int e, int& slot) {
+    if constexpr (SINK) {
+      const bool sink = e < ns;
+      return page_of(p, sink ? e : e + gap, slot) - (sink ? sp0 : pg0 - n_sp);
+    } else {
+      return page_of(p, e, slot) - pg0;
+    }
+  };
   // Invalid ids are staged as -1: loads read page 0 instead (in bounds) and the
   // compute masks the tokens, which only splits holding such an id test (any_bad).
   bool bad = false;
   {
     const int32_t* btrow = p.bt + static_cast<int64_t>(b) * p.bt_stride;
-    for (int i = tid; i <= pg1 - pg0; i += kDecThreads) {
-      const int phys = btrow[pg0 + i];
+    for (int i = tid; i <= pg1 - pg0 + n_sp; i += kDecThreads) {
+      const int phys = btrow[SINK && i < n_sp ? sp0 + i : pg0 + i - n_sp];
       const bool ok = phys >= 0 && phys < p.num_pages;
       bt_lds[i] = ok ? phys : -1;
       bad = bad || !ok;
@@ -183,8 +207,7 @@ __global__ __launch_bounds__(kDecThreads, kDecMinBlocks<DP>) void decode_split_k
   auto row_off = [&](int tok) -> int64_t {
     tok = min(tok, s_end - 1);
     int slot;
-    const int pg = page_of(p, tok, slot);
-    const int phys = max(bt_lds[pg - pg0], 0);
+    const int phys = max(bt_lds[locate(tok, slot)], 0);
     return (static_cast<int64_t>(phys) * p.page_stride + hk * p.head_stride +
             static_cast<int64_t>(slot) * D) * 2;
   };
@@ -288,7 +311,7 @@ __global__ __launch_bounds__(kDecThreads, kDecMinBlocks<DP>) void decode_split_k
       bool live = tok < s_end;  // tokens below `lo` never enter a split range
       if (any_bad && live) {
         int slot;
-        live = bt_lds[page_of(p, tok, slot) - pg0] >= 0;
+        live = bt_lds[locate(tok, slot)] >= 0;
       }
       x = live ? x : kNegInf;
       sacc[j] = x;
@@ -434,9 +457,14 @@ __global__ __launch_bounds__(256) void decode_combine_kernel(const DecodeParams 
   const int wave = threadIdx.x >> 6;
   const int n_waves = blockDim.x >> 6;
   const int L = min(max(p.lens[b], 0), p.max_len);
-  const int lo = p.window > 0 ? max(0, L - p.window) : 0;
+  int lo = p.window > 0 ? max(0, L - p.window) : 0;
+  int hi = L;
+  if (p.sinks > 0) {  // the splits number the tokens seen from 0
+    hi = L - lo + min(p.sinks, lo);
+    lo = 0;
+  }
   const int s0 = lo / p.tps;
-  const int s1 = L > 0 ? (L + p.tps - 1) / p.tps : 0;
+  const int s1 = hi > 0 ? (hi + p.tps - 1) / p.tps : 0;
   const int64_t base = (static_cast<int64_t>(b) * p.Hq + hq) * p.n_splits;
   const float* lse_row = p.ws_lse + base;
 
@@ -976,7 +1004,7 @@ void launch_decode_dp(const DecodeParams& p, bool softcap, dim3 grid, hipStream_
 }
 
 template <typename Tag>
-void launch_decode_tag(DecodeParams& p, bool softcap, dim3 grid, hipStream_t s) {
+void launch_decode_split(DecodeParams& p, bool softcap, dim3 grid, hipStream_t s) {
   if (p.D <= 32) {
     p.dp = 32;
     launch_decode_dp<Tag, 32>(p, softcap, grid, s);
@@ -992,6 +1020,15 @@ void launch_decode_tag(DecodeParams& p, bool softcap, dim3 grid, hipStream_t s) 
   } else {
     p.dp = 256;
     launch_decode_dp<Tag, 256>(p, softcap, grid, s);
+  }
+}
+
+template <typename Tag>
+void launch_decode_tag(DecodeParams& p, bool softcap, dim3 grid, hipStream_t s) {
+  if (p.sinks > 0) {
+    launch_decode_split<Sinks<Tag>>(p, softcap, grid, s);
+  } else {
+    launch_decode_split<Tag>(p, softcap, grid, s);
   }
   hipLaunchKernelGGL((decode_combine_kernel<Tag, false>), dim3(p.B * p.Hq), dim3(64), 0, s, p);
 }
@@ -1018,6 +1055,12 @@ size_t decode_workspace_bytes(int32_t batch, int32_t heads_q, int32_t head_dim,
   return rows * (static_cast<size_t>(dp_of(head_dim)) + 1) * sizeof(float);
 }
 
+int32_t decode_span(const ffa_paged_decode_args& a) {
+  if (a.window <= 0 || a.sinks <= 0) return a.max_context_len;
+  const int64_t seen = static_cast<int64_t>(a.window) + a.sinks;
+  return seen < a.max_context_len ? static_cast<int32_t>(seen) : a.max_context_len;
+}
+
 int launch_paged_decode(const ffa_paged_decode_args& a, hipStream_t stream) {
   DecodeParams p{};
   p.q = static_cast<const uint16_t*>(a.q);
@@ -1036,8 +1079,9 @@ int launch_paged_decode(const ffa_paged_decode_args& a, hipStream_t stream) {
   p.log2P = ((a.page_size & (a.page_size - 1)) == 0) ? __builtin_ctz(a.page_size) : -1;
   p.num_pages = a.num_pages;
   p.tps = decode_tokens_per_split(a.tokens_per_split);
-  p.n_splits = decode_num_splits(a.max_context_len, a.tokens_per_split);
+  p.n_splits = decode_num_splits(decode_span(a), a.tokens_per_split);
   p.window = a.window > 0 ? a.window : 0;
+  p.sinks = p.window > 0 ? a.sinks : 0;
   p.max_len = a.max_context_len;
   p.n_cg = (p.G + kCols - 1) / kCols;
   p.dp = dp_of(a.head_dim);
@@ -1108,7 +1152,7 @@ int noalloc_scratch(void** out) {
 }  // namespace
 
 int launch_paged_decode_noalloc(const ffa_paged_decode_args& a, hipStream_t stream) {
-  const size_t need = decode_workspace_bytes(a.batch, a.heads_q, a.head_dim, a.max_context_len,
+  const size_t need = decode_workspace_bytes(a.batch, a.heads_q, a.head_dim, decode_span(a),
                                              a.tokens_per_split);
   if (need > FFA_NOALLOC_SCRATCH_BYTES) return FFA_ERR_SCRATCH_LIMIT;
   void* ptr = nullptr;

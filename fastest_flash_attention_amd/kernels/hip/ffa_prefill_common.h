@@ -3,6 +3,8 @@
 // share in rows that do).
 #pragma once
 
+#include <hip/hip_runtime.h>
+
 #include "ffa_common.h"
 
 namespace ffa {
@@ -16,6 +18,9 @@ template <typename Tag>
 constexpr bool kSplitKeys = false;
 template <typename Tag>
 constexpr bool kSplitKeys<SplitKeys<Tag>> = true;
+
+template <typename Tag>
+constexpr bool kSinks<SplitKeys<Tag>> = kSinks<Tag>;
 
 // Marks the element tag of a kernel compiled for launches with a block mask.
 template <typename Tag>
@@ -36,7 +41,9 @@ constexpr float kChunkLimit = 256.0f;
 
 // Key ranges of a split launch: n0 ranges of `len` keys over the cached keys from lo0 on,
 // then the rest over the call's own keys from lo1 on (positions inside each segment;
-// len, lo0 and lo1 are multiples of the key tile).
+// len, lo0 and lo1 are multiples of the key tile). With sinks n_sink ranges come before them,
+// over the first sink_end keys (at most the sinks, and those below the window's first tile) of
+// the first segment.
 struct SplitParams {
   const uint16_t* kc;
   const uint16_t* vc;
@@ -76,6 +83,9 @@ struct PrefillParams {
   const int32_t* visited;  // reference tiles visited per row block (with kmask)
   SplitParams sp;          // split launches only
   int Do;                  // O's head dim: D, or Dv (narrow V: the zero dims are not stored)
+  // kernels marked Sinks:
+  int sinks;               // first keys seen besides the window (0 for the others)
+  int n_sink, sink_end;    // split launches: see SplitParams
 };
 
 // Row swizzles (XOR on the 16-byte chunk index) of the K and V tiles in LDS. They make
@@ -166,4 +176,9 @@ __device__ inline void ref_tile_floor(const PrefillParams& p, int row, float& ls
 }
 
 }  // namespace pf
+
+// Launches of the kernels with sinks (p.sinks > 0): whole sweeps, and key ranges.
+void launch_sinks(const pf::PrefillParams& p, int dtype, bool softcap, int grid, hipStream_t s);
+void launch_split_sinks(const pf::PrefillParams& p, bool bf16, bool softcap, int grid, hipStream_t s);
+
 }  // namespace ffa

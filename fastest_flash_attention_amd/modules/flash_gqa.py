@@ -12,8 +12,9 @@ the op runs with one KV head per q head. A cache of ``num_kv_heads`` heads is ac
 too (an extension: it is what the unrepeated path concatenates with, and it is
 ``num_heads // num_kv_heads`` times smaller).
 
-Beyond the reference: ``rotary`` (queries and keys rotated to their positions, those of a
-``kv_cache`` counted) and prompts and decode steps over a ``PagedKVCache`` (``PagedSteps``).
+Beyond the reference: ``sink_tokens`` (first keys that the window leaves visible), ``rotary``
+(queries and keys rotated to their positions, those of a ``kv_cache`` counted) and prompts and
+decode steps over a ``PagedKVCache`` (``PagedSteps``).
 """
 
 from __future__ import annotations
@@ -44,6 +45,7 @@ class FastestFlashGQA(PagedSteps, nn.Module):
         softcap: Optional[float] = None,
         sliding_window: Optional[int] = None,
         rotary: Optional[FastestFlashRotary] = None,
+        sink_tokens: int = 0,
     ):
         super().__init__()
         self.hidden_size = hidden_size
@@ -55,6 +57,7 @@ class FastestFlashGQA(PagedSteps, nn.Module):
         self.softcap = softcap
         self.sliding_window = sliding_window
         self.rotary = rotary
+        self.sink_tokens = sink_tokens
         assert num_heads % num_kv_heads == 0, "num_heads must be divisible by num_kv_heads"
         self.q_proj = nn.Linear(hidden_size, num_heads * self.head_dim, bias=bias)
         self.k_proj = nn.Linear(hidden_size, num_kv_heads * self.head_dim, bias=bias)
@@ -89,7 +92,7 @@ class FastestFlashGQA(PagedSteps, nn.Module):
         if self.training and not return_lse and kv_cache is None:
             attn = fastest_flash_attn_func(
                 q, k, v, scale=self.scale, causal=use_causal, block_size=bs or 64,
-                softcap=self.softcap, sliding_window=self.sliding_window,
+                softcap=self.softcap, **self._window(),
                 num_kv_heads=self.num_kv_heads,
             )
             lse = None
@@ -102,7 +105,7 @@ class FastestFlashGQA(PagedSteps, nn.Module):
                 kv_heads = None
             attn, lse = fastest_flash_attn_forward(
                 q, k, v, scale=self.scale, causal=use_causal, block_size=bs,
-                softcap=self.softcap, sliding_window=self.sliding_window,
+                softcap=self.softcap, **self._window(),
                 num_kv_heads=kv_heads, kv_cache=kv_cache, return_lse=return_lse,
             )
         out = self.o_proj(attn.transpose(1, 2).contiguous().view(B, S, -1))

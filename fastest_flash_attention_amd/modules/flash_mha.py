@@ -4,8 +4,9 @@ Same constructor, weights, forward signature and outputs as the reference; the
 attention core is the HIP forward. q/k/v are passed as the strided
 ``[B, H, S, D]`` views of the projections (no copies: the kernel takes any strides).
 
-Beyond the reference: ``rotary`` (queries and keys rotated to their positions, those of a
-``kv_cache`` counted) and prompts and decode steps over a ``PagedKVCache`` (``PagedSteps``).
+Beyond the reference: ``sink_tokens`` (first keys that the window leaves visible), ``rotary``
+(queries and keys rotated to their positions, those of a ``kv_cache`` counted) and prompts and
+decode steps over a ``PagedKVCache`` (``PagedSteps``).
 """
 
 from __future__ import annotations
@@ -36,6 +37,7 @@ class FastestFlashMHA(PagedSteps, nn.Module):
         softcap: Optional[float] = None,
         sliding_window: Optional[int] = None,
         rotary: Optional[FastestFlashRotary] = None,
+        sink_tokens: int = 0,
     ):
         super().__init__()
         self.hidden_size = hidden_size
@@ -49,6 +51,7 @@ class FastestFlashMHA(PagedSteps, nn.Module):
         self.softcap = softcap
         self.sliding_window = sliding_window
         self.rotary = rotary
+        self.sink_tokens = sink_tokens
         self.q_proj = nn.Linear(hidden_size, hidden_size, bias=bias)
         self.k_proj = nn.Linear(hidden_size, hidden_size, bias=bias)
         self.v_proj = nn.Linear(hidden_size, hidden_size, bias=bias)
@@ -89,13 +92,13 @@ class FastestFlashMHA(PagedSteps, nn.Module):
         if self.training and not return_lse and kv_cache is None:
             attn = fastest_flash_attn_func(
                 q, k, v, scale=self.scale, causal=use_causal, block_size=bs or 64,
-                softcap=self.softcap, sliding_window=self.sliding_window,
+                softcap=self.softcap, **self._window(),
             )
             lse = None
         else:
             attn, lse = fastest_flash_attn_forward(
                 q, k, v, scale=self.scale, causal=use_causal, block_size=bs,
-                softcap=self.softcap, sliding_window=self.sliding_window,
+                softcap=self.softcap, **self._window(),
                 kv_cache=kv_cache, return_lse=return_lse,
             )
         out = self.o_proj(attn.transpose(1, 2).contiguous().view(B, S, -1))

@@ -40,6 +40,7 @@ def fastest_flash_attn_backward(
     softcap: Optional[float] = None,
     sliding_window: Optional[int] = None,
     q_offset: int = 0,
+    sink_tokens: int = 0,
 ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Backward pass (reference ops/attention_backward.py:19-76).
 
@@ -47,6 +48,7 @@ def fastest_flash_attn_backward(
         grad_output: [B, H, S_q, D] (or [B, S_q, D])
         q, k, v, output: as in the forward (k, v may have fewer heads: GQA).
         lse: [B, H, S_q, 1] natural-log logsumexp from the forward.
+        sink_tokens: first keys that ``sliding_window`` leaves visible, as in the forward.
 
     Returns:
         (dq, dk, dv) in the dtypes and shapes of q, k, v.
@@ -92,6 +94,11 @@ def fastest_flash_attn_backward(
         raise ValueError(f"head_dim {D} > 256 is not supported by the backward kernels")
     if sliding_window is not None and int(sliding_window) <= 0:
         raise ValueError("sliding_window must be positive")
+    sink_tokens = int(sink_tokens)
+    if sink_tokens < 0:
+        raise ValueError("sink_tokens must not be negative")
+    if sliding_window is None:
+        sink_tokens = 0  # nothing is hidden that they would show
     if softcap is not None and float(softcap) <= 0.0:
         raise ValueError("softcap must be positive")
     if scale is None:
@@ -102,7 +109,7 @@ def fastest_flash_attn_backward(
     # a narrower v runs natively where the library has kernels for it (16-bit inputs,
     # head_dim 129..192, v dims <= 128 and a multiple of 8), zero-padded here otherwise
     narrow_v = (Dv < d_pad and code != _lib.FFA_DTYPE_FP32 and 128 < d_pad <= 192
-                and Dv <= 128 and Dv % 8 == 0)
+                and Dv <= 128 and Dv % 8 == 0 and not sink_tokens)
     dv_pad = Dv if narrow_v else d_pad
     if Bk != B:
         k = k.expand(B, -1, -1, -1)
@@ -141,6 +148,7 @@ def fastest_flash_attn_backward(
         a.softcap = float(softcap) if softcap is not None else 0.0
         a.dtype = code
         a.v_head_dim = Dv if narrow_v else 0
+        a.sinks = min(sink_tokens, Skv)
         ws_bytes = max(lib.ffa_attn_bwd_split_workspace_bytes(ctypes.byref(a)),
                        lib.ffa_attn_bwd_workspace_bytes(B, Hq, Sq), 16)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)

@@ -55,6 +55,7 @@ class ResolvedForward:
     squeezed: bool
     Dv: int = 0  # v's head dim (<= D; a narrower v is taken as zero-padded to D)
     cache: Optional[Tuple[torch.Tensor, torch.Tensor]] = None  # K/V ahead of k, v (in place)
+    sink_tokens: int = 0  # first keys seen besides the window (0 without a window)
 
 
 @dataclass
@@ -179,11 +180,31 @@ def _cache_fits(cache: torch.Tensor, t: torch.Tensor) -> bool:
             and cache.stride(2) < 1 << 24 and t.stride(2) < 1 << 24 and _conforms(cache))
 
 
+def _unseen_rows(cache_len: int, q_offset: int, sliding_window: Optional[int],
+                 sink_tokens: int) -> Tuple[int, int]:
+    """Rows ``[a, b)`` of a cache behind every query's window and past the sinks. Without them
+    the call is the same one with ``q_offset`` smaller by ``b - a``: what a row sees depends on
+    its distance to a key and on whether the key is a sink, and neither changes."""
+    if not sink_tokens or sliding_window is None:
+        return 0, 0
+    b = min(cache_len, q_offset - sliding_window + 1)
+    return (sink_tokens, b) if b > sink_tokens else (0, 0)
+
+
+def _cat_cache(cache: torch.Tensor, t: torch.Tensor, unseen: Tuple[int, int]) -> torch.Tensor:
+    a, b = unseen
+    parts = [cache, t] if a == b else [cache[:, :, :a], cache[:, :, b:], t]
+    return torch.cat(parts, dim=2)
+
+
 def _join_cache(r: "ResolvedForward") -> None:
     """The concatenated form of a call whose cache was kept apart."""
     if r.cache is not None:
-        r.k = torch.cat([r.cache[0], r.k], dim=2)
-        r.v = torch.cat([r.cache[1], r.v], dim=2)
+        unseen = _unseen_rows(r.cache[0].size(2), r.q_offset, r.sliding_window, r.sink_tokens)
+        r.k = _cat_cache(r.cache[0], r.k, unseen)
+        r.v = _cat_cache(r.cache[1], r.v, unseen)
+        r.q_offset -= unseen[1] - unseen[0]
+        r.S_kv -= unseen[1] - unseen[0]
         r.cache = None
 
 
@@ -205,6 +226,7 @@ def resolve_forward_args(
     kv_cache: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
     return_lse: bool = False,
     cache_in_place: bool = False,
+    sink_tokens: int = 0,
 ) -> ResolvedForward:
     """Argument resolution of the reference dispatcher (ops/attention_forward.py:65-109).
     With ``cache_in_place`` a ``kv_cache`` that fits k and v is kept apart (``cache``)
@@ -217,6 +239,15 @@ def resolve_forward_args(
         compute_dtype = config.compute_dtype
         num_kv_heads = config.num_kv_heads
         return_lse = config.return_lse
+        sink_tokens = config.sink_tokens
+
+    sink_tokens = int(sink_tokens)
+    if sink_tokens < 0:
+        raise ValueError("sink_tokens must not be negative")
+    if sliding_window is None:
+        sink_tokens = 0  # nothing is hidden that they would show
+    if sink_tokens and block_mask is not None:
+        raise ValueError("sink_tokens do not combine with a block_mask")
 
     q, k, v, squeezed = maybe_unsqueeze_head(q, k, v)
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
@@ -236,10 +267,15 @@ def resolve_forward_args(
         if cache_in_place and _cache_fits(k_cache, k) and _cache_fits(v_cache, v) \
                 and k_cache.size(2) == v_cache.size(2):
             cache = (k_cache, v_cache)
+            q_offset = S_kv - S_q
         else:
-            k = torch.cat([k_cache, k], dim=2)
-            v = torch.cat([v_cache, v], dim=2)
-        q_offset = S_kv - S_q
+            q_offset = S_kv - S_q
+            unseen = (_unseen_rows(k_cache.size(2), q_offset, sliding_window, sink_tokens)
+                      if k_cache.size(2) == v_cache.size(2) else (0, 0))
+            k = _cat_cache(k_cache, k, unseen)
+            v = _cat_cache(v_cache, v, unseen)
+            q_offset -= unseen[1] - unseen[0]
+            S_kv -= unseen[1] - unseen[0]
 
     # v may be narrower than q / k: it is then taken as zero-padded to D (the MLA
     # module's V, which the reference pads itself, modules/flash_mla.py:151-152), and
@@ -274,7 +310,7 @@ def resolve_forward_args(
         softcap=None if softcap is None else float(softcap), two_pass=bool(two_pass),
         compute_dtype=compute_dtype, block_mask=block_mask, block_q=int(bq),
         block_kv=int(bkv), return_lse=bool(return_lse), squeezed=squeezed, Dv=int(v.size(3)),
-        cache=cache,
+        cache=cache, sink_tokens=sink_tokens,
     )
 
 
@@ -308,6 +344,7 @@ def build_prefill_args(
     a.ref_block_q = r.block_q
     a.ref_block_kv = r.block_kv
     a.masked_lse_mode = 1 if r.two_pass else 0
+    a.sinks = min(r.sink_tokens, r.S_kv)
     a.dtype = dtype_code
     a.v_head_dim = r.Dv if 0 < r.Dv < r.D else 0
     a.o_head_dim = out.size(-1)
@@ -358,7 +395,7 @@ def prepare_prefill(*args, out: Optional[torch.Tensor] = None, **kwargs) -> Pref
     if r.D > 256:
         raise ValueError(f"head_dim {r.D} > 256 is not supported")
     d_pad = (r.D + 7) // 8 * 8
-    narrow = narrow_v(r.Dv, d_pad, r.q.dtype)
+    narrow = narrow_v(r.Dv, d_pad, r.q.dtype) and not r.sink_tokens  # (no such kernels)
     r.q = _conform(r.q, d_pad)
     r.k = _conform(r.k, d_pad)
     r.v = _conform(r.v, r.Dv if narrow else d_pad)
@@ -430,9 +467,12 @@ def fastest_flash_attn_forward(
     num_kv_heads: Optional[int] = None,
     kv_cache: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
     return_lse: bool = False,
+    sink_tokens: int = 0,
 ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """Forward attention on MI355X. Same signature and results as the reference's
-    ``fastest_flash_attn_forward`` (ops/attention_forward.py:23-167).
+    ``fastest_flash_attn_forward`` (ops/attention_forward.py:23-167), and ``sink_tokens``: with
+    a ``sliding_window`` the first ``sink_tokens`` keys stay visible behind it (not with a
+    ``block_mask``; the LSE is then exact, -inf for a row that sees no key).
 
     Returns ``(output, lse_or_None)``: output has q's shape and dtype; lse is fp32
     ``[B, H, S_q, 1]`` (``[B, S_q, 1]`` for 3D input), natural log.
@@ -442,7 +482,7 @@ def fastest_flash_attn_forward(
         scale=scale, causal=causal, block_size=block_size, block_mask=block_mask,
         softcap=softcap, sliding_window=sliding_window, two_pass=two_pass,
         compute_dtype=compute_dtype, num_kv_heads=num_kv_heads, kv_cache=kv_cache,
-        return_lse=return_lse,
+        return_lse=return_lse, sink_tokens=sink_tokens,
     )
     launch_prefill(call)
     output, lse = call.out, call.lse
@@ -466,7 +506,8 @@ def forward_token_major(
     if D % 8 != 0:
         out, lse = fastest_flash_attn_forward(q, k, v, **kwargs)
         return out.transpose(1, 2).contiguous(), lse
-    width = v.size(3) if drop_zero_dims and narrow_v(v.size(3), D, q.dtype) else D
+    narrow = narrow_v(v.size(3), D, q.dtype) and not kwargs.get("sink_tokens")
+    width = v.size(3) if drop_zero_dims and narrow else D
     tokens = torch.empty(B, S, H, width, dtype=q.dtype, device=q.device)
     call = prepare_prefill(q, k, v, out=tokens.transpose(1, 2), **kwargs)
     launch_prefill(call)

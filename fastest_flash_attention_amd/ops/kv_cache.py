@@ -84,10 +84,10 @@ def set_append_pages(a: _lib.PagedAppendArgs, table: Sequence[int], start: int, 
 
 def check_page_ids(block_tables: torch.Tensor, context_lens: torch.Tensor, page_size: int,
                    num_pages: int, max_context_len: int,
-                   sliding_window: Optional[int] = None) -> None:
+                   sliding_window: Optional[int] = None, sink_tokens: int = 0) -> None:
     """Raise IndexError if a page id the lengths reach lies outside ``[0, num_pages)``:
     entry j of row b is used when ``j * page_size < min(context_lens[b],
-    max_context_len)`` and it holds a token of the window. One device reduction and a host
+    max_context_len)`` and it holds a token of the window or a sink. One device reduction and a host
     sync."""
     if block_tables.numel() == 0:
         return
@@ -95,7 +95,7 @@ def check_page_ids(block_tables: torch.Tensor, context_lens: torch.Tensor, page_
     first = torch.arange(block_tables.size(1), device=block_tables.device)[None, :] * page_size
     used = first < lens[:, None]
     if sliding_window is not None:
-        used &= first + page_size > lens[:, None] - sliding_window
+        used &= (first + page_size > lens[:, None] - sliding_window) | (first < sink_tokens)
     bad = used & ((block_tables < 0) | (block_tables >= num_pages))
     if bool(bad.any()):
         b, j = (int(x) for x in bad.nonzero()[0])
@@ -104,7 +104,7 @@ def check_page_ids(block_tables: torch.Tensor, context_lens: torch.Tensor, page_
 
 
 def _paged_decode_fp32(q3, k_pages, v_pages, block_tables, context_lens, scale, softcap,
-                       sliding_window, return_lse, max_context_len):
+                       sliding_window, sink_tokens, return_lse, max_context_len):
     """Decode over fp32 pools: per sequence, ``ffa_paged_gather`` of its pages and one
     ``ffa_prefill_fwd`` on the fp32 MFMA kernel with the query at position L - 1 (the
     reference's get_kv + forward, ops/kv_cache.py:208-232, in fp32 as it computes).
@@ -116,7 +116,8 @@ def _paged_decode_fp32(q3, k_pages, v_pages, block_tables, context_lens, scale, 
     lens = [min(n, int(max_context_len))
             for n in context_lens.to(torch.int64).clamp(min=0).tolist()]
     bt = block_tables  # int32, contiguous, wide enough for max_context_len (checked)
-    check_page_ids(bt, context_lens, page_size, P_total, int(max_context_len), sliding_window)
+    check_page_ids(bt, context_lens, page_size, P_total, int(max_context_len), sliding_window,
+                   sink_tokens)
     out = torch.zeros((B, Hq, D), dtype=torch.float32, device=q3.device)
     lse = (torch.full((B, Hq), float("-inf"), dtype=torch.float32, device=q3.device)
            if return_lse else None)
@@ -141,8 +142,8 @@ def _paged_decode_fp32(q3, k_pages, v_pages, block_tables, context_lens, scale, 
         _lib.launch(lib.ffa_paged_gather, g, q3.device)
         call = prepare_prefill(q3[b, :, None, :].unsqueeze(0), k.unsqueeze(0), v.unsqueeze(0),
                                scale=scale, causal=True, softcap=softcap,
-                               sliding_window=sliding_window, num_kv_heads=Hkv,
-                               return_lse=return_lse)
+                               sliding_window=sliding_window, sink_tokens=sink_tokens,
+                               num_kv_heads=Hkv, return_lse=return_lse)
         call.args.q_offset = L - 1  # the query is the sequence's last token
         launch_prefill(call)
         out[b] = call.out[0, :, 0, :D]
@@ -172,6 +173,7 @@ def fastest_flash_paged_decode(
     tokens_per_split: Optional[int] = None,
     workspace: Optional[torch.Tensor] = None,
     check_block_tables: bool = False,
+    sink_tokens: int = 0,
 ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """One decode step for a batch of paged sequences.
 
@@ -191,7 +193,9 @@ def fastest_flash_paged_decode(
     position ``context_lens[b] - 1``: the result equals the reference
     ``fastest_flash_attn_forward(q_b, k_new, v_new, kv_cache=get_kv(b)[:L-1],
     num_kv_heads=Hkv, ...)`` for the last token (ops/attention_forward.py:82-96,
-    ops/kv_cache.py:208-232). Returns ``(O, lse)`` with O shaped like q and lse fp32
+    ops/kv_cache.py:208-232). With ``sliding_window`` it sees its last ``sliding_window``
+    tokens and its first ``sink_tokens``; table entries of pages without any of them are not
+    read. Returns ``(O, lse)`` with O shaped like q and lse fp32
     ``[B, Hq]`` (``[B, Hq, 1, 1]`` for 4D q) or None.
     """
     squeeze = q.dim() == 3
@@ -237,9 +241,11 @@ def fastest_flash_paged_decode(
                     f"fastest_flash_attention_amd paged decode runs on ROCm tensors only; "
                     f"{name} is on {t.device}"
                 )
+    if sink_tokens < 0:
+        raise ValueError("sink_tokens must not be negative")
     if q3.dtype == torch.float32:
         out, lse = _paged_decode_fp32(q3, k_pages, v_pages, block_tables, context_lens,
-                                      scale, softcap, sliding_window, return_lse,
+                                      scale, softcap, sliding_window, sink_tokens, return_lse,
                                       max_context_len)
         if not squeeze:
             out = out.unsqueeze(2)
@@ -253,20 +259,23 @@ def fastest_flash_paged_decode(
         q3 = q3.contiguous() if not q3.is_contiguous() else q3.clone()
     if check_block_tables:
         check_page_ids(block_tables, context_lens, page_size, P_total, max_context_len,
-                       sliding_window)
+                       sliding_window, sink_tokens)
     if scale is None:
         scale = 1.0 / math.sqrt(D)
     if sliding_window is not None and int(sliding_window) <= 0:
         raise ValueError("sliding_window must be positive")
     if softcap is not None and float(softcap) <= 0.0:
         raise ValueError("softcap must be positive")
+    span = max_context_len  # the most tokens a sequence sees
+    if sliding_window is not None and sink_tokens:
+        span = min(span, int(sliding_window) + sink_tokens)
     if tokens_per_split is None:
-        tokens_per_split = _auto_tokens_per_split(B, Hkv, max_context_len)
+        tokens_per_split = _auto_tokens_per_split(B, Hkv, span)
 
     lib = _lib.load()
     out = torch.empty((B, Hq, D), dtype=q3.dtype, device=q3.device)
     lse = torch.empty((B, Hq), dtype=torch.float32, device=q3.device) if return_lse else None
-    need = int(lib.ffa_paged_decode_workspace_bytes(B, Hq, D, max_context_len, tokens_per_split))
+    need = int(lib.ffa_paged_decode_workspace_bytes(B, Hq, D, span, tokens_per_split))
     if workspace is None or workspace.numel() * workspace.element_size() < need:
         workspace = torch.empty(max(need, 4), dtype=torch.uint8, device=q3.device)
 
@@ -297,6 +306,7 @@ def fastest_flash_paged_decode(
     a.scale = float(scale)
     a.softcap = float(softcap) if softcap is not None else 0.0
     a.dtype = code
+    a.sinks = min(sink_tokens, max_context_len)
     _lib.launch(lib.ffa_paged_decode_fwd, a, q3.device)
     if not squeeze:
         out = out.unsqueeze(2)
@@ -756,15 +766,17 @@ class PagedKVCache(PageBook):
         softcap: Optional[float] = None,
         sliding_window: Optional[int] = None,
         return_lse: bool = False,
+        sink_tokens: int = 0,
     ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
         """Decode attention of ``q`` (``[B, Hq, D]``, one token per sequence of
         ``seq_ids``) over the cached tokens, read in place from the pages."""
-        self._check_seen(seq_ids, sliding_window, 0)
+        self._check_seen(seq_ids, sliding_window, sink_tokens)
         bt, lens = self.block_tables(seq_ids)
         max_len = max([0] + [self.sequences[s]["len"] for s in seq_ids if s in self.sequences])
         return fastest_flash_paged_decode(
             q, self.k_pages, self.v_pages, bt, lens, scale=scale, softcap=softcap,
             sliding_window=sliding_window, return_lse=return_lse, max_context_len=max_len,
+            sink_tokens=sink_tokens,
         )
 
     @property

@@ -58,7 +58,7 @@
 extern "C" {
 #endif
 
-#define FFA_ABI_VERSION 14
+#define FFA_ABI_VERSION 15
 
 typedef enum ffa_status {
   FFA_OK = 0,
@@ -171,6 +171,11 @@ typedef struct ffa_prefill_args {
      small) such a call without a cache runs unsplit. 16-byte aligned. */
   void* workspace;
   size_t workspace_bytes;
+  int32_t sinks;  /* >= 0: with a window, the first `sinks` keys stay visible to every row
+                     (causal: from their own position on). Rows then have their exact LSE,
+                     -inf without a visible key, as with masked_lse_mode = 1. Not with a block
+                     mask (FFA_ERR_INVALID_ARG) nor a narrower v
+                     (FFA_ERR_UNSUPPORTED_HEAD_DIM). */
 } ffa_prefill_args;
 
 int ffa_prefill_fwd(const ffa_prefill_args* args, void* stream);
@@ -320,6 +325,10 @@ typedef struct ffa_paged_decode_args {
   float scale;                   /* any finite value */
   float softcap;                 /* <= 0: none; else finite */
   int32_t dtype;                 /* FFA_DTYPE_BF16 or FFA_DTYPE_FP16 */
+  int32_t sinks;                 /* >= 0: with a window, the first `sinks` tokens stay visible
+                                    too; the splits then cut the tokens seen, and the
+                                    workspace of max_context_len = min(max_context_len,
+                                    window + sinks) is enough */
 } ffa_paged_decode_args;
 
 /* Split count per sequence the decode entry point uses for these sizes. */
@@ -614,12 +623,13 @@ typedef struct ffa_attn_bwd_args {
                                and dv have v_head_dim < head_dim dims, v taken as
                                zero-padded to head_dim as in ffa_prefill_fwd (dout and o
                                keep head_dim dims); the same support rule. */
+  int32_t sinks;            /* >= 0: as in ffa_prefill_fwd (not with a narrower v) */
 } ffa_attn_bwd_args;
 
 size_t ffa_attn_bwd_workspace_bytes(int32_t batch, int32_t heads_q, int32_t seqlen_q);
 /* Workspace of this call with which its dK/dV sweeps may be cut over more workgroups (few
  * and uneven ones otherwise); at least ffa_attn_bwd_workspace_bytes, with which it runs too,
- * and at most 90 MB more.
+ * and at most 90 MB more (180 MB with sinks).
  * Reads sizes and options only. 0 for sizes that ffa_attn_bwd refuses. */
 size_t ffa_attn_bwd_split_workspace_bytes(const ffa_attn_bwd_args* args);
 int ffa_attn_bwd(const ffa_attn_bwd_args* args, void* stream);
