@@ -82,6 +82,8 @@ size_t plan_dkv_parts(BwdParams& p, int32_t dtype) {
   return bytes + static_cast<size_t>(units) * p.n_cut * p.n_part * tile_bytes;
 }
 
+constexpr int kSinkGroups = 512;  // workgroups that the sinks' rows are split over
+
 void fill_bwd_sizes(const ffa_attn_bwd_args& a, BwdParams& p) {
   p.B = a.batch;
   p.Hq = a.heads_q;
@@ -99,15 +101,41 @@ void fill_bwd_sizes(const ffa_attn_bwd_args& a, BwdParams& p) {
   p.n_kt = (a.seqlen_kv + kDkvKeys - 1) / kDkvKeys;
   p.sinks = clamp_sinks(a.sinks, p.window, a.q_offset, a.seqlen_q);
   p.sinks = p.sinks < a.seqlen_kv ? p.sinks : a.seqlen_kv;
-  p.n_skt = (p.sinks + kDkvKeys - 1) / kDkvKeys;
+  p.n_skt = p.sinks / kDkvKeys;
+  p.sink0 = p.n_skt * kDkvKeys;
+  if (a.dtype == FFA_DTYPE_FP32) {  // 32-key workgroups anyway: all of the sinks in parts
+    p.n_skt = 0;
+    p.sink0 = 0;
+  }
+  p.n_skb = (p.sinks - p.sink0 + 31) / 32;
+  p.n_part_k = 1;
+  p.part_len_k = 0x7fffffff;
 }
+
+// Rows of the sinks' 32-key blocks over workgroups: sets n_part_k and part_len_k, returns the bytes
+// of the partials. A part has at least two row tiles for each of its four waves; there are parts
+// for about two workgroups per CU, and none (each block's rows stay whole) with 256 blocks and
+// more, so at most 512 partial blocks of 32 keys (32 MB at head_dim 256).
+size_t plan_sink_parts(BwdParams& p, int32_t dtype) {
+  const int64_t blocks = static_cast<int64_t>(p.B) * p.Hkv * p.n_skb;
+  if (blocks == 0 || blocks >= 256 || (dtype == FFA_DTYPE_FP32 && p.D > 128)) return 0;
+  const int64_t items = static_cast<int64_t>(p.ratio) * ((p.Sq + kDkvRows - 1) / kDkvRows);
+  int64_t parts = kSinkGroups / blocks;
+  parts = parts < items / 8 ? parts : items / 8;
+  if (parts < 2) return 0;
+  p.part_len_k = static_cast<int>((items + parts - 1) / parts);
+  p.n_part_k = static_cast<int>((items + p.part_len_k - 1) / p.part_len_k);
+  return static_cast<size_t>(blocks) * p.n_part_k * 64 * p.D * sizeof(float);
+}
+
 
 }  // namespace
 
 size_t attn_bwd_split_workspace_bytes(const ffa_attn_bwd_args& a) {
   BwdParams p{};
   fill_bwd_sizes(a, p);
-  return attn_bwd_workspace_bytes(a.batch, a.heads_q, a.seqlen_q) + plan_dkv_parts(p, a.dtype);
+  return attn_bwd_workspace_bytes(a.batch, a.heads_q, a.seqlen_q) + plan_dkv_parts(p, a.dtype) +
+         plan_sink_parts(p, a.dtype);
 }
 
 int launch_attn_bwd(const ffa_attn_bwd_args& a, hipStream_t stream) {
@@ -165,16 +193,18 @@ int launch_attn_bwd(const ffa_attn_bwd_args& a, hipStream_t stream) {
   p.lse2 = ws;
   p.di = ws + rows;
   const size_t stats = attn_bwd_workspace_bytes(a.batch, a.heads_q, a.seqlen_q);
+  const size_t sink_parts = plan_sink_parts(p, a.dtype);
   const size_t parts = plan_dkv_parts(p, a.dtype);
-  p.part = ws + stats / sizeof(float);
-  if (parts == 0 || a.workspace_bytes < stats + parts) {
-    p.n_part = p.n_part_s = 1;
-    p.part_len = p.part_len_s = 0x7fffffff;
-  }
-  // (the partials of the sinks' tiles follow the others')
+  // behind the statistics: the partials of the sinks' blocks, of the window's tiles, of the sinks'
+  p.part_k = ws + stats / sizeof(float);
+  p.part = p.part_k + sink_parts / sizeof(float);
   p.part_s = p.part;
   if (p.n_part > 1) {
     p.part_s += static_cast<int64_t>(a.batch) * a.heads_kv * p.n_cut * p.n_part * kDkvKeys * (p.D + p.Dv);
+  }
+  if (a.workspace_bytes < stats + sink_parts + parts) {  // whole sweeps need none
+    p.n_part = p.n_part_s = p.n_part_k = 1;
+    p.part_len = p.part_len_s = p.part_len_k = 0x7fffffff;
   }
 
   const int64_t grid_pre = rows / 32;
@@ -182,7 +212,8 @@ int launch_attn_bwd(const ffa_attn_bwd_args& a, hipStream_t stream) {
   const int64_t kv_units = static_cast<int64_t>(a.batch) * a.heads_kv;
   const int64_t grid_win = (p.n_kt - p.n_skt) * p.n_part * kv_units;  // workgroups of the window's tiles
   const int64_t grid_dkv = grid_win + static_cast<int64_t>(p.n_skt) * p.n_part_s * kv_units;
-  if (grid_pre > 0x7fffffff || grid_dq > 0x7fffffff || grid_dkv > 0x7fffffff) {
+  if (grid_pre > 0x7fffffff || grid_dq > 0x7fffffff || grid_dkv > 0x7fffffff ||
+      kv_units * p.n_skb * p.n_part_k > 0x7fffffff) {
     return FFA_ERR_TOO_LARGE;
   }
   if (grid_pre == 0 || grid_dq == 0) return FFA_OK;

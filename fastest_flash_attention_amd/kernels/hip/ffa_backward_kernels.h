@@ -88,10 +88,14 @@ struct BwdParams {
   // those of key tiles [cut_first, cut_first + n_cut)
   int n_part, part_len, cut_first, n_cut;
   float* part;  // [B * Hkv][n_cut][n_part][128 keys][D + Dv] fp32 dK | dV of cut sweeps
-  // kernels marked Sinks: the first keys, which every row sees besides its window. Their n_skt
-  // key tiles have sweeps over all rows, cut into n_part_s parts of part_len_s tiles
+  // kernels marked Sinks: the first `sinks` keys, which every row sees besides its window. Whole
+  // key tiles of them (n_skt) are swept by all rows in the dK/dV kernel, cut into n_part_s parts
+  // of part_len_s tiles; the sinks past those, from sink0 on, have a kernel of their own
+  // (bwd_sink_kernel): n_skb blocks of 32 keys, rows in n_part_k parts of part_len_k tiles
   int sinks, n_skt, n_part_s, part_len_s;
   float* part_s;  // [B * Hkv][n_skt][n_part_s][128 keys][D + Dv]
+  int sink0, n_skb, n_part_k, part_len_k;
+  float* part_k;  // [B * Hkv][n_skb][n_part_k][32 keys][2 D] (n_part_k > 1)
 };
 
 }  // namespace bwd
@@ -120,7 +124,7 @@ __host__ __device__ inline void dkv_rows(const BwdParams& p, int kt, int& first,
   const int k_last = (k0 + kDkvKeys < p.Skv ? k0 + kDkvKeys : p.Skv) - 1;
   const int q_lo = p.causal && k0 > p.q_offset ? k0 - p.q_offset : 0;
   int q_hi = p.Sq;
-  if (p.window > 0 && !(SINK && k0 < p.sinks)) {  // (a tile of sinks: every row)
+  if (p.window > 0 && !(SINK && kt < p.n_skt)) {  // (a tile of sinks: every row)
     const int64_t hi = static_cast<int64_t>(k_last) + p.window - p.q_offset;
     q_hi = hi < q_hi ? static_cast<int>(hi) : q_hi;
   }
@@ -345,10 +349,10 @@ constexpr int kBwdMinBlocks = DP <= 128 ? 2 : 1;
 // the rule and what it measured). A variant of its own: the part's bounds cost the uncut
 // kernel 2-4 % (8 % at head_dim 64), and at head_dim 256 they spill.
 //
-// SINK (Tag = Sinks<...>): the key tiles of the sinks are swept by every row, the others by a
-// window's: S / 32 tiles a head against (W + 128) / 32, by a few workgroups. So they come first
-// in the grid, cut into parts (plan_dkv_parts); of their four waves those without a sink leave
-// the rows past their window out.
+// SINK (Tag = Sinks<...>): whole tiles of sinks are swept by every row, the others by a window's:
+// S / 32 tiles a head against (W + 128) / 32, by a few workgroups. So they come first in the grid,
+// cut into parts (plan_dkv_parts). The sinks past the last whole tile are left to bwd_sink_kernel:
+// this kernel computes their window's share along with their tile's and does not store it.
 template <typename Tag, int DP, int DV, bool SOFTCAP, bool CUT>
 __global__ __launch_bounds__(kThreads, kBwdMinBlocks<DP>) void bwd_dkdv_kernel(const BwdParams p) {
   using S = BShape<DP>;   // Q, K, dK
@@ -371,26 +375,32 @@ __global__ __launch_bounds__(kThreads, kBwdMinBlocks<DP>) void bwd_dkdv_kernel(c
   const int l32 = lane & 31;
   const int g = lane >> 5;
 
+  constexpr bool SINK = kSinks<Tag>;
   int bh, kt;  // causal: low key tiles are seen by the most rows (heaviest first)
   int part = 0;
-  constexpr bool SINK = kSinks<Tag>;
-  const int per_s = SINK ? p.n_skt * p.n_part_s : 0;  // workgroups of a unit's sink tiles
-  const int n_first = SINK ? per_s * p.B * p.Hkv : 0;
-  const bool sink_tile = SINK && static_cast<int>(blockIdx.x) < n_first;
-  auto n_part = [&]() { return SINK && sink_tile ? p.n_part_s : p.n_part; };
-  auto part_len = [&]() { return SINK && sink_tile ? p.part_len_s : p.part_len; };
-  if (sink_tile) {
-    bh = __builtin_amdgcn_readfirstlane(blockIdx.x / per_s);
-    kt = __builtin_amdgcn_readfirstlane(blockIdx.x % per_s);
+  bool sink_tile = false;
+  int n_part = p.n_part, part_len = p.part_len;
+  if constexpr (!SINK) {
+    bwd_item(blockIdx.x, CUT ? p.n_kt * p.n_part : p.n_kt, p.xcd_group_dkv, p.xcd_remap_dkv, bh, kt);
   } else {
-    const int n_kt = SINK ? p.n_kt - p.n_skt : p.n_kt;
-    bwd_item(blockIdx.x, CUT ? n_kt * n_part() : n_kt, p.xcd_group_dkv, p.xcd_remap_dkv, bh, kt, n_first);
+    const int per = p.n_skt * p.n_part_s;  // workgroups of a unit's sink tiles
+    const int before = per * p.B * p.Hkv;
+    sink_tile = static_cast<int>(blockIdx.x) < before;
+    if (sink_tile) {
+      bh = __builtin_amdgcn_readfirstlane(blockIdx.x / per);
+      kt = __builtin_amdgcn_readfirstlane(blockIdx.x % per);
+      n_part = p.n_part_s;
+      part_len = p.part_len_s;
+    } else {
+      const int n_kt = p.n_kt - p.n_skt;
+      bwd_item(blockIdx.x, CUT ? n_kt * n_part : n_kt, p.xcd_group_dkv, p.xcd_remap_dkv, bh, kt, before);
+    }
   }
   if constexpr (CUT) {
-    part = kt % n_part();
-    kt /= n_part();
+    part = kt % n_part;
+    kt /= n_part;
   }
-  if (SINK && !sink_tile) kt += p.n_skt;
+  if constexpr (SINK) kt += sink_tile ? 0 : p.n_skt;
   const int b = bh / p.Hkv;
   const int hk = bh - b * p.Hkv;
   const int D = p.D;
@@ -405,9 +415,9 @@ __global__ __launch_bounds__(kThreads, kBwdMinBlocks<DP>) void bwd_dkdv_kernel(c
   dkv_rows<SINK>(p, kt, qt_begin, ntq);
   const int nit = ntq * p.ratio;
   // this workgroup's part of the sweep (every part but the first may be empty)
-  const bool cut = CUT && nit > part_len();
-  const int it_begin = CUT ? part * part_len() : 0;
-  const int it_end = CUT ? min(nit, it_begin + part_len()) : nit;
+  const bool cut = CUT && nit > part_len;
+  const int it_begin = CUT ? part * part_len : 0;
+  const int it_end = CUT ? min(nit, it_begin + part_len) : nit;
   if (CUT && part > 0 && it_begin >= nit) return;
 
   const float c = SOFTCAP ? p.cap_mul : p.score_mul;
@@ -492,8 +502,8 @@ __global__ __launch_bounds__(kThreads, kBwdMinBlocks<DP>) void bwd_dkdv_kernel(c
     if (q0 + kDkvRows <= Sq) {
 #pragma unroll
       for (int j = 0; j < LPT; ++j) {
-        load_lds16_async(is_qb, q_off[j], lds_addr(&q_lds[buf][(4 * j + wave) * 512]));
-        if (j < LPTV) load_lds16_async(is_db, do_off[j], lds_addr(&do_lds[buf][(4 * j + wave) * 512]));
+        load_lds16_async<SINK>(is_qb, q_off[j], lds_addr(&q_lds[buf][(4 * j + wave) * 512]));
+        if (j < LPTV) load_lds16_async<SINK>(is_db, do_off[j], lds_addr(&do_lds[buf][(4 * j + wave) * 512]));
       }
     } else {
       // rows past Sq re-read row Sq - 1: their lse2 is +inf, so P = dS = 0
@@ -502,10 +512,10 @@ __global__ __launch_bounds__(kThreads, kBwdMinBlocks<DP>) void bwd_dkdv_kernel(c
         const int row = ((4 * j + wave) * 64 + lane) / S::CPR;
         const int over = max(0, q0 + row - (Sq - 1));
         const uint32_t qback = static_cast<uint32_t>(over * p.q_ss * 2);
-        load_lds16_async(is_qb, q_off[j] - qback, lds_addr(&q_lds[buf][(4 * j + wave) * 512]));
+        load_lds16_async<SINK>(is_qb, q_off[j] - qback, lds_addr(&q_lds[buf][(4 * j + wave) * 512]));
         if constexpr (!NARROW) {
           const uint32_t dback = static_cast<uint32_t>(over * p.do_ss * 2);
-          load_lds16_async(is_db, do_off[j] - dback, lds_addr(&do_lds[buf][(4 * j + wave) * 512]));
+          load_lds16_async<SINK>(is_db, do_off[j] - dback, lds_addr(&do_lds[buf][(4 * j + wave) * 512]));
         }
       }
       if constexpr (NARROW) {
@@ -514,7 +524,7 @@ __global__ __launch_bounds__(kThreads, kBwdMinBlocks<DP>) void bwd_dkdv_kernel(c
           const int row = ((4 * j + wave) * 64 + lane) / SV::CPR;
           const int over = max(0, q0 + row - (Sq - 1));
           const uint32_t dback = static_cast<uint32_t>(over * p.do_ss * 2);
-          load_lds16_async(is_db, do_off[j] - dback, lds_addr(&do_lds[buf][(4 * j + wave) * 512]));
+          load_lds16_async<SINK>(is_db, do_off[j] - dback, lds_addr(&do_lds[buf][(4 * j + wave) * 512]));
         }
       }
     }
@@ -569,7 +579,7 @@ __global__ __launch_bounds__(kThreads, kBwdMinBlocks<DP>) void bwd_dkdv_kernel(c
     const int q0_abs = p.q_offset + q0;
     if (!wave_live) continue;
     if (p.causal && kw0 > q0_abs + kDkvRows - 1) continue;
-    if (p.window > 0 && kw0 + 31 < q0_abs - p.window + 1 && !(SINK && kw0 < p.sinks)) continue;
+    if (p.window > 0 && !(SINK && sink_tile) && kw0 + 31 < q0_abs - p.window + 1) continue;
     const uint16_t* ql = q_lds[buf];
     const uint16_t* dl = do_lds[buf];
     const float* st = st_lds[buf];
@@ -636,7 +646,7 @@ __global__ __launch_bounds__(kThreads, kBwdMinBlocks<DP>) void bwd_dkdv_kernel(c
       const int qa0 = q0_abs + 4 * g;
       const int lo = p.causal ? key - qa0 : -0x7fffffff;
       // (window clamped on the host; a sink is seen past it)
-      const int hi = p.window > 0 && !(SINK && key < p.sinks) ? key + p.window - 1 - qa0 : 0x7fffffff;
+      const int hi = p.window > 0 && !(SINK && sink_tile) ? key + p.window - 1 - qa0 : 0x7fffffff;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int off = 8 * (r >> 2) + (r & 3);
@@ -673,9 +683,13 @@ __global__ __launch_bounds__(kThreads, kBwdMinBlocks<DP>) void bwd_dkdv_kernel(c
 
   if (cut) {
     if (key < p.Skv) {
-      const int64_t tile = sink_tile ? (static_cast<int64_t>(bh) * p.n_skt + kt) * n_part() + part
-                                     : (static_cast<int64_t>(bh) * p.n_cut + (kt - p.cut_first)) * n_part() + part;
-      float* row = (sink_tile ? p.part_s : p.part) + (tile * kDkvKeys + (key - k0)) * (D + Dv);
+      int64_t tile = (static_cast<int64_t>(bh) * p.n_cut + (kt - p.cut_first)) * p.n_part + part;
+      float* base = p.part;
+      if (SINK && sink_tile) {
+        tile = (static_cast<int64_t>(bh) * p.n_skt + kt) * p.n_part_s + part;
+        base = p.part_s;
+      }
+      float* row = base + (tile * kDkvKeys + (key - k0)) * (D + Dv);
 #pragma unroll
       for (int db = 0; db < S::DB; ++db) {
 #pragma unroll
@@ -694,7 +708,7 @@ __global__ __launch_bounds__(kThreads, kBwdMinBlocks<DP>) void bwd_dkdv_kernel(c
     }
     return;
   }
-  if (wave_live && key < p.Skv) {
+  if (wave_live && key < p.Skv && !(SINK && !sink_tile && key < p.sinks)) {
     store_rows<Tag, DP>(p.dk + b * p.dk_sb + hk * p.dk_sh + static_cast<int64_t>(key) * p.dk_ss,
                         dkacc, p.scale, D, g);
     store_rows<Tag, DV>(p.dv + b * p.dv_sb + hk * p.dv_sh + static_cast<int64_t>(key) * p.dv_ss,
@@ -741,6 +755,7 @@ __global__ __launch_bounds__(kThreads) void bwd_dkdv_sum_kernel(const BwdParams 
       }
     }
     const int64_t key = static_cast<int64_t>(kt) * kDkvKeys + r;
+    if (kt >= p.n_skt && key < p.sinks) continue;  // bwd_sink_kernel's
     const bool is_k = d0 < p.D;
     const float mul = is_k ? p.scale : 1.0f;
     uint16_t* dst = is_k ? p.dk + b * p.dk_sb + hk * p.dk_sh + key * p.dk_ss + d0
@@ -1277,7 +1292,7 @@ __device__ inline void f32_pds(const BwdParams& p, float s, float dp, float l2, 
 }
 
 // Sum the partial accumulators of the four waves in LDS (wave order 0, 1, 2, 3) into
-// wave 0's registers. `red` holds 3 x 64 x NA floats and no tile is in use any more.
+// wave 0's registers. `red` holds 3 x 64 x 16 NA floats and no tile is in use any more.
 template <int NA>
 __device__ inline void wave_reduce4(float* red, f32x16 (&acc)[NA], int wave, int lane) {
   __syncthreads();  // every wave is done with its tiles
@@ -1316,6 +1331,308 @@ __device__ inline void store_acc_row_f32(float* row, const f32x16* acc, float mu
   }
 }
 
+// ---------------------------------------------------------------------------------
+// 2b. dK, dV of sinks past the last whole key tile of them: 32 keys per workgroup, all rows.
+// ---------------------------------------------------------------------------------
+// A few sinks meet every query row, so their gradients are one pass over Q and dO with little to
+// compute: bound by reading those two once (from HBM or the Infinity Cache) and, with the rows
+// split over the chip, by latency. The waves of a workgroup share the 32 keys (K in
+// registers, V in LDS) and take row tiles in turn, each through a private LDS ring without
+// barriers: two stages up to head_dim 128, one above (LDS). Their sums meet in LDS at the end;
+// parts of the rows, one workgroup each, in the workspace (bwd_sink_sum_kernel), both in a fixed
+// order. In the 128-key dK/dV kernel the same sweep kept one wave of four busy and took as long
+// as the whole window: SINKNUMBERS
+template <int DP>
+constexpr int kSinkStages = DP <= 128 ? 2 : 1;
+// What a launch computes: 1 dV, 2 dK, 3 both. At head_dim 256 two launches: 256 accumulators per
+// lane beside the row tiles' operands spill.
+template <int DP>
+constexpr int kSinkSums = DP <= 192 ? 3 : 1;
+
+template <typename Tag, int DP, bool SOFTCAP, int SUMS>
+__global__ __launch_bounds__(kThreads, 1) void bwd_sink_kernel(const BwdParams p) {
+  using S = BShape<DP>;
+  using E = Elem<Tag>;
+  constexpr int TILE = kDkvRows * DP;
+  constexpr int LPT = TILE / 8 / 64;  // loads per lane of one tile
+  constexpr int NB = kSinkStages<DP>;
+  constexpr int NW = 4;
+  constexpr bool SUM_V = (SUMS & 1) != 0;
+  constexpr bool SUM_K = (SUMS & 2) != 0;
+  static_assert((NW - 1) * 64 * 16 * S::DB * 4 <= NW * NB * 2 * TILE * 2, "the waves' sums fit in the tiles");
+  __shared__ __attribute__((aligned(1024))) uint16_t tiles[NW][NB][2][TILE];  // each wave's Q, dO
+  __shared__ __attribute__((aligned(1024))) float st_lds[NW][NB][256];        // lse2, D_i of 32 rows
+  __shared__ __attribute__((aligned(1024))) uint16_t v_lds[TILE];            // V of the 32 keys
+
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = tid & 63;
+  const int l32 = lane & 31;
+  const int g = lane >> 5;
+  // key blocks of one part (the same rows) have consecutive ids
+  const int kb = blockIdx.x % p.n_skb;
+  const int part = (blockIdx.x / p.n_skb) % p.n_part_k;
+  const int bh = blockIdx.x / (p.n_skb * p.n_part_k);
+  const int b = bh / p.Hkv;
+  const int hk = bh - b * p.Hkv;
+  const int D = p.D;
+  const int Sq = p.Sq;
+  const int k0 = p.sink0 + 32 * kb;
+  const int key = k0 + l32;
+
+  // row tiles [qt0, qt0 + ntq) of every query head of the group; this workgroup's share
+  const int qt0 = p.causal ? max(0, k0 - p.q_offset) / kDkvRows : 0;
+  const int ntq = max((Sq + kDkvRows - 1) / kDkvRows - qt0, 0);
+  const int it_begin = part * p.part_len_k;
+  const int it_end = min(ntq * p.ratio, it_begin + p.part_len_k);
+
+  u32x4 kreg[S::KS];
+  load_row_operand<DP>(p.k + b * p.k_sb + hk * p.k_sh + static_cast<int64_t>(min(key, p.Skv - 1)) * p.k_ss, D, g,
+                       kreg);
+  if constexpr (SUM_K) {
+    const uint16_t* vb = p.v + b * p.v_sb + hk * p.v_sh;
+    for (int pos = tid; pos < TILE / 8; pos += kThreads) {
+      const int row = pos / S::CPR;
+      const int cq = (pos - row * S::CPR) ^ bswz<DP>(row);
+      u32x4 val = {0u, 0u, 0u, 0u};  // dims past D
+      if (8 * cq < D) val = *reinterpret_cast<const u32x4*>(vb + static_cast<int64_t>(min(k0 + row, p.Skv - 1)) * p.v_ss + 8 * cq);
+      *reinterpret_cast<u32x4*>(&v_lds[8 * pos]) = val;
+    }
+  }
+  const float c = SOFTCAP ? p.cap_mul : p.score_mul;
+
+  uint32_t q_off[LPT], do_off[LPT];
+#pragma unroll
+  for (int j = 0; j < LPT; ++j) {
+    const int pos = j * 64 + lane;
+    const int row = pos / S::CPR;
+    const int cq = min((pos - row * S::CPR) ^ bswz<DP>(row), (D >> 3) - 1);
+    q_off[j] = static_cast<uint32_t>(row * p.q_ss * 2 + cq * 16);
+    do_off[j] = static_cast<uint32_t>(row * p.do_ss * 2 + cq * 16);
+  }
+  // the wave's next item: tile is_qi of head is_r of the group
+  int is_r = 0;
+  int is_qi = it_begin + wave;
+  if (ntq > 0) {
+    is_r = is_qi / ntq;
+    is_qi -= is_r * ntq;
+  }
+  auto issue = [&](int buf) {
+    const int hq = hk * p.ratio + is_r;
+    const int q0 = (qt0 + is_qi) * kDkvRows;
+    const char* qb = reinterpret_cast<const char*>(p.q + b * p.q_sb + hq * p.q_sh + static_cast<int64_t>(q0) * p.q_ss);
+    const char* db = reinterpret_cast<const char*>(p.dout + b * p.do_sb + hq * p.do_sh + static_cast<int64_t>(q0) * p.do_ss);
+    const bool whole = q0 + kDkvRows <= Sq;
+#pragma unroll
+    for (int j = 0; j < LPT; ++j) {
+      uint32_t qo = q_off[j], dof = do_off[j];
+      if (!whole) {  // rows past Sq re-read row Sq - 1: their lse2 is +inf, so P = dS = 0
+        const int over = max(0, q0 + (j * 64 + lane) / S::CPR - (Sq - 1));
+        qo -= static_cast<uint32_t>(over * p.q_ss * 2);
+        dof -= static_cast<uint32_t>(over * p.do_ss * 2);
+      }
+      load_lds16_async(qb, qo, lds_addr(&tiles[wave][buf][0][j * 512]));
+      load_lds16_async(db, dof, lds_addr(&tiles[wave][buf][1][j * 512]));
+    }
+    // lanes 0-7: lse2 of the rows, lanes 8-15: D_i (the others repeat them)
+    const float* src = ((lane & 8) ? p.di : p.lse2) + (static_cast<int64_t>(b) * p.Hq + hq) * p.sq_pad + q0 + 4 * (lane & 7);
+    load_lds16_async(src, lds_addr(&st_lds[wave][buf][0]));
+    is_qi += NW;
+    while (is_qi >= ntq) {
+      is_qi -= ntq;
+      ++is_r;
+    }
+  };
+
+  const int a_rd0 = row_rd0<DP>(lane);
+  int t_lo0, t_hi0;
+  tr_offsets<DP>(lane, t_lo0, t_hi0);
+  f32x16 dkacc[S::DB], dvacc[S::DB];
+#pragma unroll
+  for (int db = 0; db < S::DB; ++db) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      dkacc[db][r] = 0.0f;
+      dvacc[db][r] = 0.0f;
+    }
+    if constexpr (DP > 64) {
+      if constexpr (SUM_K) pin_agpr(dkacc[db]);
+      if constexpr (SUM_V) pin_agpr(dvacc[db]);
+    }
+  }
+  wait_vmcnt0();    // K is in registers: the waits below count tile loads alone
+  __syncthreads();  // V is in LDS
+
+  const int n_my = it_end > it_begin + wave ? (it_end - it_begin - wave + NW - 1) / NW : 0;
+  int cur_qi = is_qi;
+  if (n_my > 0) issue(0);
+  for (int i = 0; i < n_my; ++i) {
+    const int buf = NB == 2 ? i & 1 : 0;
+    const int next_qi = is_qi;
+    if (NB == 2 && i + 1 < n_my) {
+      wait_lgkmcnt0();  // the stage's last reads are done before it is filled again
+      issue(buf ^ 1);
+      wait_vmcnt<2 * LPT + 1>();
+    } else {
+      wait_vmcnt0();
+    }
+    wave_lds_order();
+    const int q0_abs = p.q_offset + (qt0 + cur_qi) * kDkvRows;
+    cur_qi = next_qi;
+    const uint16_t* ql = tiles[wave][buf][0];
+    const uint16_t* dl = tiles[wave][buf][1];
+    const float* st = st_lds[wave][buf];
+    const int a_rd = opaque(a_rd0);
+    const int t_lo = opaque(t_lo0);
+    const int t_hi = opaque(t_hi0);
+    f32x16 sacc, dpacc;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      sacc[r] = 0.0f;
+      dpacc[r] = 0.0f;
+    }
+    // operands one k-step ahead of the MFMAs that consume them
+    auto rd = [&](const uint16_t* tile, int ks) { return *reinterpret_cast<const u32x4*>(tile + row_rd<DP>(a_rd, ks)); };
+    u32x4 aq = rd(ql, 0);
+    u32x4 ad, bv;
+    if constexpr (SUM_K) {
+      ad = rd(dl, 0);
+      bv = rd(v_lds, 0);
+    }
+#pragma unroll
+    for (int ks = 0; ks < S::KS; ++ks) {
+      u32x4 aq_n, ad_n, bv_n;
+      if (ks + 1 < S::KS) {
+        aq_n = rd(ql, ks + 1);
+        if constexpr (SUM_K) {
+          ad_n = rd(dl, ks + 1);
+          bv_n = rd(v_lds, ks + 1);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      sacc = E::mfma32(aq, kreg[ks], sacc);
+      if constexpr (SUM_K) dpacc = E::mfma32(ad, bv, dpacc);
+      if (ks + 1 < S::KS) {
+        aq = aq_n;
+        if constexpr (SUM_K) {
+          ad = ad_n;
+          bv = bv_n;
+        }
+      }
+    }
+    float pv[16], dsv[16];
+    const int lo = p.causal ? key - (q0_abs + 4 * g) : -0x7fffffff;  // first row (offset) that sees the key
+#pragma unroll
+    for (int ii = 0; ii < 4; ++ii) {
+      const f32x4 l2 = *reinterpret_cast<const f32x4*>(st + 8 * ii + 4 * g);
+      const f32x4 di = *reinterpret_cast<const f32x4*>(st + 32 + 8 * ii + 4 * g);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = 4 * ii + j;
+        float pr, ds;
+        if constexpr (SOFTCAP) {
+          const float t = tanh_fast(sacc[r] * p.tanh_mul);
+          pr = fast_exp2(fmaf(t, c, -l2[j]));
+          ds = pr * (dpacc[r] - di[j]) * fmaf(-t, t, 1.0f);
+        } else {
+          pr = fast_exp2(fmaf(sacc[r], c, -l2[j]));
+          ds = pr * (dpacc[r] - di[j]);
+        }
+        const bool ok = 8 * ii + j >= lo;
+        pv[r] = ok ? pr : 0.0f;
+        dsv[r] = ok ? ds : 0.0f;
+      }
+    }
+#pragma unroll
+    for (int cc = 0; cc < 2; ++cc) {
+      const int e0 = 8 * cc;
+      const u32x4 bp = {E::pack2(pv[e0 + 0], pv[e0 + 1]), E::pack2(pv[e0 + 2], pv[e0 + 3]),
+                        E::pack2(pv[e0 + 4], pv[e0 + 5]), E::pack2(pv[e0 + 6], pv[e0 + 7])};
+      const u32x4 bs = {E::pack2(dsv[e0 + 0], dsv[e0 + 1]), E::pack2(dsv[e0 + 2], dsv[e0 + 3]),
+                        E::pack2(dsv[e0 + 4], dsv[e0 + 5]), E::pack2(dsv[e0 + 6], dsv[e0 + 7])};
+#pragma unroll
+      for (int db = 0; db < S::DB; ++db) {
+        if constexpr (SUM_V) dvacc[db] = E::mfma32(tr_operand<DP>(dl + 16 * cc * DP, t_lo, t_hi, db), bp, dvacc[db]);
+        if constexpr (SUM_K) dkacc[db] = E::mfma32(tr_operand<DP>(ql + 16 * cc * DP, t_lo, t_hi, db), bs, dkacc[db]);
+      }
+    }
+    if constexpr (DP > 64) {
+#pragma unroll
+      for (int db = 0; db < S::DB; ++db) {
+        if constexpr (SUM_K) pin_agpr(dkacc[db]);
+        if constexpr (SUM_V) pin_agpr(dvacc[db]);
+      }
+    }
+    if (NB == 1 && i + 1 < n_my) {
+      wait_lgkmcnt0();
+      issue(0);
+    }
+  }
+
+  float* red = reinterpret_cast<float*>(&tiles[0][0][0][0]);
+  float* row = p.part_k + (((static_cast<int64_t>(bh) * p.n_skb + kb) * p.n_part_k + part) * 32 + l32) * 2 * D;
+  const bool mine = wave == 0 && key < p.sinks;
+  if constexpr (SUM_K) {
+    wave_reduce4<S::DB>(red, dkacc, wave, lane);
+    if (mine && p.n_part_k == 1) {
+      store_rows<Tag, DP>(p.dk + b * p.dk_sb + hk * p.dk_sh + static_cast<int64_t>(key) * p.dk_ss, dkacc, p.scale, D, g);
+    } else if (mine) {
+      store_acc_row_f32<S::DB>(row, dkacc, 1.0f, D, g);
+    }
+  }
+  if constexpr (SUM_V) {
+    wave_reduce4<S::DB>(red, dvacc, wave, lane);
+    if (mine && p.n_part_k == 1) {
+      store_rows<Tag, DP>(p.dv + b * p.dv_sb + hk * p.dv_sh + static_cast<int64_t>(key) * p.dv_ss, dvacc, 1.0f, D, g);
+    } else if (mine) {
+      store_acc_row_f32<S::DB>(row + D, dvacc, 1.0f, D, g);
+    }
+  }
+}
+
+// dK and dV of those keys: the sum of the parts in part order. One thread per 4 dims of a key.
+// F32Tag: fp32 gradients, of whole 32-key blocks (the fp32 kernel computes a block's keys past the
+// sinks along with them).
+template <typename Tag>
+__global__ __launch_bounds__(kThreads) void bwd_sink_sum_kernel(const BwdParams p) {
+  const int bh = blockIdx.x / p.n_skb;
+  const int kb = blockIdx.x - bh * p.n_skb;
+  const int b = bh / p.Hkv;
+  const int hk = bh - b * p.Hkv;
+  const int per_row = p.D >> 1;  // 4-dim pieces of dK | dV
+  const int keys = min(32, (std::is_same_v<Tag, F32Tag> ? p.Skv : p.sinks) - p.sink0 - 32 * kb);
+  const float* base = p.part_k + static_cast<int64_t>(blockIdx.x) * p.n_part_k * 64 * p.D;
+  for (int idx = blockIdx.y * kThreads + threadIdx.x; idx < keys * per_row; idx += gridDim.y * kThreads) {
+    const int r = idx / per_row;
+    const int d0 = 4 * (idx - r * per_row);
+    const float* src = base + static_cast<int64_t>(r) * 2 * p.D + d0;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int i0 = 0; i0 < p.n_part_k; i0 += 8) {
+      f32x4 x[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        x[u] = *reinterpret_cast<const f32x4*>(src + static_cast<int64_t>(min(i0 + u, p.n_part_k - 1)) * 64 * p.D);
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        if (i0 + u < p.n_part_k) acc += x[u];
+      }
+    }
+    const int64_t key = p.sink0 + 32 * kb + r;
+    const bool is_k = d0 < p.D;
+    const float mul = is_k ? p.scale : 1.0f;
+    const int64_t at = is_k ? b * p.dk_sb + hk * p.dk_sh + key * p.dk_ss + d0
+                            : b * p.dv_sb + hk * p.dv_sh + key * p.dv_ss + (d0 - p.D);
+    uint16_t* const out = is_k ? p.dk : p.dv;
+    if constexpr (std::is_same_v<Tag, F32Tag>) {
+      *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(out) + at) = acc * mul;
+    } else {
+      *reinterpret_cast<u32x2*>(out + at) = u32x2{Elem<Tag>::pack2(acc[0] * mul, acc[1] * mul),
+                                                  Elem<Tag>::pack2(acc[2] * mul, acc[3] * mul)};
+    }
+  }
+}
+
 // dQ: two workgroups per CU at head_dim 64. dK / dV: one (its 4 waves hold K, V, dK and dV
 // of 32 keys plus a prefetched tile at head_dim 64; at 128 the tile is loaded when it is
 // needed), except at head_dim 64 with more than 384 workgroups: without the prefetched tile
@@ -1345,11 +1662,25 @@ __global__ __launch_bounds__(kThreads, (TWO ? 2 : 1)) void bwd_f32m_dkdv_kernel(
   float* dt = qt + kM32 * PITCH;
   float* st = stl[wave];
 
-  // heaviest key blocks (causal: block 0 sees every row) first, all heads at once
+  // heaviest key blocks (causal: block 0 sees every row) first, all heads at once; blocks that
+  // hold sinks, which all rows see, ahead of them in parts of part_len_k items
   const int units = p.B * p.Hkv;
   int rank = blockIdx.x;
-  const int n_all = units * ((p.Skv + kM32 - 1) / kM32);
-  if (TWO && p.causal && n_all <= 512) rank = paired_rank(rank, 256, n_all);
+  int part = 0;
+  int n_all = units * ((p.Skv + kM32 - 1) / kM32);
+  bool sink_block = false;
+  if constexpr (SINK) {
+    const int n_first = units * p.n_skb * p.n_part_k;
+    sink_block = rank < n_first;
+    if (sink_block) {
+      part = rank / units % p.n_part_k;
+      rank = rank / units / p.n_part_k * units + rank % units;
+    } else {
+      rank += units * p.n_skb - n_first;
+    }
+  } else {
+    if (TWO && p.causal && n_all <= 512) rank = paired_rank(rank, 256, n_all);
+  }
   const int kb = rank / units;
   const int bh = rank - kb * units;
   const int b = bh / p.Hkv;
@@ -1364,7 +1695,8 @@ __global__ __launch_bounds__(kThreads, (TWO ? 2 : 1)) void bwd_f32m_dkdv_kernel(
                                 : p.Sq;
   const int j_lo = q_lo / kM32;
   const int nj = q_hi > q_lo ? (q_hi + kM32 - 1) / kM32 - j_lo : 0;
-  const int n_items = p.ratio * nj;
+  const int n_items = SINK && sink_block ? min(p.ratio * nj, (part + 1) * p.part_len_k) : p.ratio * nj;
+  const int first_item = SINK && sink_block ? part * p.part_len_k : 0;
 
   const float* qf = reinterpret_cast<const float*>(p.q);
   const float* dof = reinterpret_cast<const float*>(p.dout);
@@ -1397,8 +1729,8 @@ __global__ __launch_bounds__(kThreads, (TWO ? 2 : 1)) void bwd_f32m_dkdv_kernel(
     statn = (g == 0 ? p.lse2 : p.di)[ws];
   };
   constexpr bool PREFETCH = DP <= 64 && !TWO;
-  if (PREFETCH && wave < n_items) fetch(wave);
-  for (int i = wave; i < n_items; i += 4) {
+  if (PREFETCH && first_item + wave < n_items) fetch(first_item + wave);
+  for (int i = first_item + wave; i < n_items; i += 4) {
     const int q0 = (j_lo + i % nj) * kM32;
     if (!PREFETCH) fetch(i);
     qn.store(qt, lane);
@@ -1459,6 +1791,14 @@ __global__ __launch_bounds__(kThreads, (TWO ? 2 : 1)) void bwd_f32m_dkdv_kernel(
   }
 
   wave_reduce4<2 * DB>(lds, acc, wave, lane);
+  if (SINK && sink_block && p.n_part_k > 1) {
+    if (wave == 0 && key < p.Skv) {
+      float* row = p.part_k + (((static_cast<int64_t>(bh) * p.n_skb + kb) * p.n_part_k + part) * 32 + l32) * 2 * D;
+      store_acc_row_f32<DB>(row, acc, 1.0f, D, g);
+      store_acc_row_f32<DB>(row + D, acc + DB, 1.0f, D, g);
+    }
+    return;
+  }
   if (wave == 0 && key < p.Skv) {
     float* dkr = reinterpret_cast<float*>(p.dk) + b * p.dk_sb + hk * p.dk_sh + static_cast<int64_t>(key) * p.dk_ss;
     float* dvr = reinterpret_cast<float*>(p.dv) + b * p.dv_sb + hk * p.dv_sh + static_cast<int64_t>(key) * p.dv_ss;
@@ -1609,7 +1949,7 @@ __global__ __launch_bounds__(kThreads, kF32mDqBlocks<DP>) void bwd_f32m_dq_kerne
 
 template <int DP, bool SOFTCAP, bool SINK>
 void launch_f32m_dp(const BwdParams& p, hipStream_t s) {
-  const int grid_dkv = p.B * p.Hkv * ((p.Skv + kM32 - 1) / kM32);
+  const int grid_dkv = p.B * p.Hkv * ((p.Skv + kM32 - 1) / kM32 + (SINK ? p.n_skb * (p.n_part_k - 1) : 0));
   const int grid_dq = p.B * p.Hq * ((p.Sq + kM32 - 1) / kM32);
   if (grid_dkv > 0) {
     bool two = false;
@@ -1621,6 +1961,9 @@ void launch_f32m_dp(const BwdParams& p, hipStream_t s) {
     }
     if (!two) {
       hipLaunchKernelGGL((bwd_f32m_dkdv_kernel<DP, SOFTCAP, false, SINK>), dim3(grid_dkv), dim3(kThreads), 0, s, p);
+    }
+    if (SINK && p.n_part_k > 1) {
+      hipLaunchKernelGGL((bwd_sink_sum_kernel<F32Tag>), dim3(p.B * p.Hkv * p.n_skb, 4), dim3(kThreads), 0, s, p);
     }
   }
   hipLaunchKernelGGL((bwd_f32m_dq_kernel<DP, SOFTCAP, SINK>), dim3(grid_dq), dim3(kThreads), 0, s, p);
@@ -1663,6 +2006,18 @@ void launch_main(const BwdParams& p, int grid_dkv, int grid_dq, hipStream_t s) {
     }
     if (!cut) {
       hipLaunchKernelGGL((bwd_dkdv_kernel<Tag, DP, DV, SOFTCAP, false>), dim3(grid_dkv), dim3(kThreads), 0, s, p);
+    }
+  }
+  if constexpr (kSinks<Tag>) {
+    if (p.n_skb > 0) {
+      const dim3 grid(p.B * p.Hkv * p.n_skb * p.n_part_k);
+      hipLaunchKernelGGL((bwd_sink_kernel<Plain, DP, SOFTCAP, kSinkSums<DP>>), grid, dim3(kThreads), 0, s, p);
+      if constexpr (kSinkSums<DP> == 1) {
+        hipLaunchKernelGGL((bwd_sink_kernel<Plain, DP, SOFTCAP, 2>), grid, dim3(kThreads), 0, s, p);
+      }
+      if (p.n_part_k > 1) {
+        hipLaunchKernelGGL((bwd_sink_sum_kernel<Plain>), dim3(p.B * p.Hkv * p.n_skb, 4), dim3(kThreads), 0, s, p);
+      }
     }
   }
   hipLaunchKernelGGL((bwd_dq_kernel<Tag, DP, DV, SOFTCAP>), dim3(grid_dq), dim3(kThreads), 0, s, p);

@@ -259,10 +259,26 @@ __device__ inline void load_lds16(const void* src, void* lds_base) {
 // publishes the tile) and must not overwrite LDS another wave may still be reading.
 // Address = wave-uniform `base` (SGPR pair) + per-lane 32-bit byte offset `voff`;
 // `lds_base` is the LDS byte address (wave-uniform), carried in M0.
+//
+// A vector memory instruction must not read an SGPR within five wait states of a VALU instruction
+// that writes it, and the compiler keeps that distance for its own loads only: where it restores a
+// spilled base with v_readlane right before this asm, the load goes to a wrong address. GUARD
+// copies the base in the asm (a scalar move waits for the VALU, and the load for the move): for
+// kernels that spill their bases. The others are held to the distance by
+// tests/test_asm_hazards.py.
+template <bool GUARD = false>
 __device__ inline void load_lds16_async(const void* base, uint32_t voff, uint32_t lds_base) {
-  asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(base),
-               "{m0}"(__builtin_amdgcn_readfirstlane(lds_base))
-               : "memory");
+  if constexpr (GUARD) {
+    uint64_t copy;
+    asm volatile("s_mov_b64 %0, %2\n\tglobal_load_lds_dwordx4 %1, %0"
+                 : "=&s"(copy)
+                 : "v"(voff), "s"(base), "{m0}"(__builtin_amdgcn_readfirstlane(lds_base))
+                 : "memory");
+  } else {
+    asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(base),
+                 "{m0}"(__builtin_amdgcn_readfirstlane(lds_base))
+                 : "memory");
+  }
 }
 
 // Same, with a per-lane 64-bit address (sources that need not share a 4 GiB window).
