@@ -31,7 +31,11 @@ namespace {
 // with parts of one even share 1, 12/12, 2048, 128 not causal: 137 / 151, so it stays uncut.
 //
 // With sinks the same share counts all tiles; those of the sinks (n_skt of them, swept by every
-// row) and the window's are cut apart: SINKCUTS
+// row) and the window's are cut apart. The sweeps of the sinks are few and come first, so they are
+// cut from 1.5 parts on; us with 2.5 / 1.5, and with 1.5 at parts of one even share:
+//   1, 16/16, 4096, 128, window 500, 1024 sinks   283 / 213, 246
+//   2, 16/4, 3000, 128, window 500, 256 sinks     202 / 202, 218
+//   4, 32/8, 4096, 64, window 256, 128 sinks      415 / 415, 333
 size_t plan_dkv_parts(BwdParams& p, int32_t dtype) {
   p.n_part = p.n_part_s = 1;
   p.part_len = p.part_len_s = 0x7fffffff;
@@ -53,7 +57,7 @@ size_t plan_dkv_parts(BwdParams& p, int32_t dtype) {
   const int64_t even = (3 * total * units + 2 * slots - 1) / (2 * slots);
   size_t bytes = 0;
   int64_t len = even < 16 ? 16 : even;
-  if (2 * most_s > 5 * len) {
+  if (2 * most_s > 3 * len) {
     if (most_s > 16 * len) len = (most_s + 15) / 16;  // at most 16 parts
     p.n_part_s = static_cast<int>((most_s + len - 1) / len);
     p.part_len_s = static_cast<int>(len);
@@ -68,7 +72,8 @@ size_t plan_dkv_parts(BwdParams& p, int32_t dtype) {
   // concave function of the key tile (q_hi - q_lo of dkv_rows), so they follow one another
   // and average at least (len + most) / 2: with len at least 1.5 even shares that is at most
   // 4/3 slots partial tiles, 90 MB at head_dim 128 (683 of 128 KB), whatever the lengths
-  // of the sequences. (Sinks: as many again for theirs, whose sweeps are all of the rows.)
+  // of the sequences. (Sweeps of sinks are equal, with at
+  // most 4/3 parts for each `len` of them: at most 8/9 slots, 60 MB.)
   int end = 0;
   p.cut_first = p.n_kt;
   for (int kt = p.n_skt; kt < p.n_kt; ++kt) {
@@ -82,7 +87,7 @@ size_t plan_dkv_parts(BwdParams& p, int32_t dtype) {
   return bytes + static_cast<size_t>(units) * p.n_cut * p.n_part * tile_bytes;
 }
 
-constexpr int kSinkGroups = 512;  // workgroups that the sinks' rows are split over
+constexpr int kSinkGroups = 256;  // workgroups that the sinks' rows are split over
 
 void fill_bwd_sizes(const ffa_attn_bwd_args& a, BwdParams& p) {
   p.B = a.batch;

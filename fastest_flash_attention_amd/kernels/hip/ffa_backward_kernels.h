@@ -1340,8 +1340,11 @@ __device__ inline void store_acc_row_f32(float* row, const f32x16* acc, float mu
 // registers, V in LDS) and take row tiles in turn, each through a private LDS ring without
 // barriers: two stages up to head_dim 128, one above (LDS). Their sums meet in LDS at the end;
 // parts of the rows, one workgroup each, in the workspace (bwd_sink_sum_kernel), both in a fixed
-// order. In the 128-key dK/dV kernel the same sweep kept one wave of four busy and took as long
-// as the whole window: SINKNUMBERS
+// order. In the 128-key dK/dV kernel the same sweep keeps one wave of four busy at the cost of a
+// full one. Whole backward on MI355X, us, sinks there (cut into parts) / here / window alone, B, Hq/Hkv,
+// S, D, window, sinks, bf16:
+//   1, 32/8, 8192, 128, 1024, 4    625 / 560 /        2, 32/8, 2011, 128, 512, 4   206 / 214 / 184
+//   1, 8/8, 8192, 256, 2048, 64    832 / 641 / 566    1, 16/16, 4096, 64, 1000, 4  111 / 106 / 93
 template <int DP>
 constexpr int kSinkStages = DP <= 128 ? 2 : 1;
 // What a launch computes: 1 dV, 2 dK, 3 both. At head_dim 256 two launches: 256 accumulators per

@@ -143,14 +143,24 @@ def _bwd_bytes(B, Hq, Hkv, S, D, window, sinks, off=0, dtype=0):
             - lib.ffa_attn_bwd_workspace_bytes(B, Hq, S))
 
 
-def test_backward_cuts_the_sinks_sweeps():
+@pytest.mark.parametrize("D,dtype", [(128, 0), (256, 0), (64, 2)])
+def test_backward_cuts_the_sinks_rows(D, dtype):
+    """The rows of 32-key blocks of sinks go over the chip: whole parts per block and KV head."""
+    block = 32 * 2 * D * 4
+    got = _bwd_bytes(1, 32, 8, 8192, D, 1024, 4, dtype=dtype)
+    assert got == 256 * block  # 8 KV heads, one block each: 32 parts
+    assert _bwd_bytes(1, 32, 8, 8192, D, 1024, 40, dtype=dtype) == 256 * block  # two blocks: 16 parts
+    assert _bwd_bytes(1, 32, 8, 8192, D, 1024, 0, dtype=dtype) == 0
+    assert _bwd_bytes(32, 32, 8, 8192, D, 1024, 4, dtype=dtype) == 0  # blocks enough without
+    assert _bwd_bytes(1, 8, 8, 200, D, 64, 4, dtype=dtype) == 0       # seven row tiles a block
+
+
+def test_backward_cuts_the_sinks_tiles():
+    """Sweeps of whole 128-key tiles of sinks are cut from 1.5 parts on."""
     tile = 128 * 2 * 128 * 4
-    got = _bwd_bytes(1, 32, 8, 8192, 128, 1024, 4)
-    assert got > 0 and got % (8 * tile) == 0  # whole parts of one key tile per KV head
-    assert _bwd_bytes(1, 32, 8, 8192, 128, 1024, 0) == 0
-    assert _bwd_bytes(1, 32, 8, 8192, 128, 1024, 4, dtype=2) == 0  # fp32 sweeps are not cut
-    assert _bwd_bytes(1, 32, 8, 8192, 256, 1024, 4) == 0           # nor those past head_dim 192
-    assert _bwd_bytes(8, 32, 8, 8192, 128, 1024, 4) >= 0
+    got = _bwd_bytes(1, 16, 16, 4096, 128, 500, 1024)
+    assert got == 16 * 8 * 2 * tile
+    assert _bwd_bytes(1, 32, 8, 8192, 256, 1024, 128) == 0  # not past head_dim 192
 
 
 @pytest.mark.parametrize("seed", range(40))
