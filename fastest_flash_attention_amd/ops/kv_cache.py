@@ -35,7 +35,7 @@ import torch
 from ..kernels import _lib
 from .attention_forward import launch_prefill, prepare_prefill
 from .pages import PageBook, device_ints
-from .rotary import check_frequencies, check_magnitude
+from .rotary import check_frequencies, check_magnitude, in_and_out
 
 
 def _auto_tokens_per_split(batch: int, heads_kv: int, max_len: int) -> int:
@@ -374,7 +374,7 @@ def fastest_flash_paged_append(
     device = k.device
     for name, t in (("k", k), ("v", v), ("q", q), ("k_pages", k_pages), ("v_pages", v_pages),
                     ("block_tables", block_tables), ("positions", positions), ("counts", counts)):
-        if t is None:
+        if t is None or (t is not k and t.device == device):
             continue
         if t.device.type != "cuda":
             raise RuntimeError("fastest_flash_attention_amd paged append runs on ROCm tensors only; "
@@ -391,19 +391,13 @@ def fastest_flash_paged_append(
     k, v = (t if D == 1 or t.stride(3) == 1 else t.contiguous() for t in (k, v))
     out = None
     if q is not None:
-        q = q if D == 1 or q.stride(3) == 1 else q.contiguous()
-        out = torch.empty_like(q)
-        if D > 1 and out.stride(3) != 1:
-            out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        q, out, a.q_stride[:], a.q_out_stride[:] = in_and_out(q)
         a.q, a.q_out, a.heads_q = q.data_ptr(), out.data_ptr(), q.size(1)
-        a.q_stride[:] = list(q.stride()[:3])
-        a.q_out_stride[:] = list(out.stride()[:3])
     block_tables, positions = block_tables.contiguous(), positions.contiguous()
     counts = counts.contiguous() if counts is not None else None
     a.k_pages, a.v_pages = k_pages.data_ptr(), v_pages.data_ptr()
     a.k_new, a.v_new = k.data_ptr(), v.data_ptr()
-    a.k_new_stride[:] = list(k.stride()[:3])
-    a.v_new_stride[:] = list(v.stride()[:3])
+    a.k_new_stride[:], a.v_new_stride[:] = k.stride()[:3], v.stride()[:3]
     a.block_tables, a.positions = block_tables.data_ptr(), positions.data_ptr()
     a.counts = counts.data_ptr() if counts is not None else None
     a.block_table_stride = block_tables.size(1)

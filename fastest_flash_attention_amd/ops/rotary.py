@@ -99,8 +99,18 @@ def check_magnitude(magnitude: float) -> float:
     return magnitude
 
 
-def _strides(t: torch.Tensor) -> list[int]:
-    return list(t.stride()[:3])
+def in_and_out(t: torch.Tensor):
+    """The tensor as the kernel reads it, its output, and their strides of batch, head and token."""
+    stride = t.stride()
+    if stride[3] != 1 and t.size(3) > 1:
+        t = t.contiguous()
+        stride = t.stride()
+    out = torch.empty_like(t)
+    out_stride = out.stride()
+    if out_stride[3] != 1 and t.size(3) > 1:
+        out = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+        out_stride = out.stride()
+    return t, out, stride[:3], out_stride[:3]
 
 
 def _rotate(q: Optional[torch.Tensor], k: Optional[torch.Tensor], inv_freq: torch.Tensor,
@@ -109,24 +119,14 @@ def _rotate(q: Optional[torch.Tensor], k: Optional[torch.Tensor], inv_freq: torc
     """One launch over 4D tensors (either may be None); outputs in the inputs' memory order."""
     x = q if q is not None else k
     a = _lib.RotaryArgs()
-    outs = []
-    keep = []  # copies of inputs without a unit dim stride, until the launch
-    for name, t in (("q", q), ("k", k)):
-        if t is None:
-            outs.append(None)
-            continue
-        if t.size(3) > 1 and t.stride(3) != 1:
-            t = t.contiguous()
-            keep.append(t)
-        out = torch.empty_like(t)
-        if out.size(3) > 1 and out.stride(3) != 1:
-            out = torch.empty(t.shape, dtype=t.dtype, device=t.device)
-        setattr(a, name, t.data_ptr())
-        setattr(a, name + "_out", out.data_ptr())
-        getattr(a, name + "_stride")[:] = _strides(t)
-        getattr(a, name + "_out_stride")[:] = _strides(out)
-        setattr(a, "heads_" + name, t.size(1))
-        outs.append(out)
+    a.batch, _, a.seqlen, a.head_dim = x.shape
+    q_out = k_out = None
+    if q is not None:  # (q and k: kept until the launch where they are copies)
+        q, q_out, a.q_stride[:], a.q_out_stride[:] = in_and_out(q)
+        a.q, a.q_out, a.heads_q = q.data_ptr(), q_out.data_ptr(), q.size(1)
+    if k is not None:
+        k, k_out, a.k_stride[:], a.k_out_stride[:] = in_and_out(k)
+        a.k, a.k_out, a.heads_k = k.data_ptr(), k_out.data_ptr(), k.size(1)
     a.inv_freq = inv_freq.data_ptr()
     a.q_offset = q_offset
     if positions is not None:
@@ -134,16 +134,13 @@ def _rotate(q: Optional[torch.Tensor], k: Optional[torch.Tensor], inv_freq: torc
         a.position_bytes = positions.element_size()
         a.position_stride[:] = [positions.stride(0) if positions.size(0) > 1 else 0,
                                 positions.stride(1)]
-    a.batch = x.size(0)
-    a.seqlen = x.size(2)
-    a.head_dim = x.size(3)
     a.rotary_dim = 2 * inv_freq.numel()
-    a.interleaved = 1 if interleaved else 0
-    a.inverse = 1 if inverse else 0
+    a.interleaved = interleaved
+    a.inverse = inverse
     a.magnitude = magnitude
     a.dtype = _lib.dtype_code(x.dtype, allow_fp32=True)
     _lib.launch(_lib.load().ffa_rotary, a, x.device)
-    return outs[0], outs[1]
+    return q_out, k_out
 
 
 class _Rotary(torch.autograd.Function):
@@ -165,7 +162,9 @@ class _Rotary(torch.autograd.Function):
         if not ctx.needs_input_grad[1]:
             dk = None
         if dq is not None or dk is not None:
-            dq, dk = _Rotary.apply(dq, dk, inv_freq, positions, *ctx.how, not ctx.inverse)
+            # (an autograd call of its own only where the gradient is differentiated again)
+            rotate = _Rotary.apply if torch.is_grad_enabled() else _rotate
+            dq, dk = rotate(dq, dk, inv_freq, positions, *ctx.how, not ctx.inverse)
         return dq, dk, None, None, None, None, None, None
 
 
