@@ -106,12 +106,10 @@ void fill_bwd_sizes(const ffa_attn_bwd_args& a, BwdParams& p) {
   p.n_kt = (a.seqlen_kv + kDkvKeys - 1) / kDkvKeys;
   p.sinks = clamp_sinks(a.sinks, p.window, a.q_offset, a.seqlen_q);
   p.sinks = p.sinks < a.seqlen_kv ? p.sinks : a.seqlen_kv;
-  p.n_skt = p.sinks / kDkvKeys;
+  // Whole key tiles of sinks: swept in the dK/dV kernel where it is compiled for cut sweeps, else
+  // (fp32: 32-key workgroups) in blocks like the other sinks.
+  p.n_skt = a.dtype == FFA_DTYPE_FP32 || p.D > kCutMaxDim ? 0 : p.sinks / kDkvKeys;
   p.sink0 = p.n_skt * kDkvKeys;
-  if (a.dtype == FFA_DTYPE_FP32) {  // 32-key workgroups anyway: all of the sinks in parts
-    p.n_skt = 0;
-    p.sink0 = 0;
-  }
   p.n_skb = (p.sinks - p.sink0 + 31) / 32;
   p.n_part_k = 1;
   p.part_len_k = 0x7fffffff;

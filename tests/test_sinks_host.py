@@ -160,7 +160,7 @@ def test_backward_cuts_the_sinks_tiles():
     tile = 128 * 2 * 128 * 4
     got = _bwd_bytes(1, 16, 16, 4096, 128, 500, 1024)
     assert got == 16 * 8 * 2 * tile
-    assert _bwd_bytes(1, 32, 8, 8192, 256, 1024, 128) == 0  # not past head_dim 192
+    assert _bwd_bytes(1, 32, 8, 8192, 256, 1024, 128) == 32 * 8 * 32 * 2 * 256 * 4  # blocks past head_dim 192
 
 
 @pytest.mark.parametrize("seed", range(40))
