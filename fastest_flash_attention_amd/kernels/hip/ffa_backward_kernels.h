@@ -12,8 +12,8 @@
 // head sum over the q heads of its group. A row whose LSE is -inf (no visible key in
 // the two-pass forward) contributes nothing (P = 0).
 //
-// Three launches on the caller's stream (four where dK/dV sweeps are cut into parts), no
-// atomics (results are run-to-run deterministic):
+// Three launches on the caller's stream (four where dK/dV sweeps are cut into parts, up to three
+// more with sinks: 2b and the sums of parts), no atomics (results are run-to-run deterministic):
 //   1. bwd_pre_kernel   lse2 = lse * log2e (+inf for -inf rows and the padding rows up
 //                       to the next 128-row boundary) and D_i, both fp32, into the
 //                       workspace [B * Hq][Sq_pad].
@@ -1343,7 +1343,7 @@ __device__ inline void store_acc_row_f32(float* row, const f32x16* acc, float mu
 // order. In the 128-key dK/dV kernel the same sweep keeps one wave of four busy at the cost of a
 // full one. Whole backward on MI355X, us, sinks there (cut into parts) / here / window alone, B, Hq/Hkv,
 // S, D, window, sinks, bf16:
-//   1, 32/8, 8192, 128, 1024, 4    625 / 560 /        2, 32/8, 2011, 128, 512, 4   206 / 214 / 184
+//   1, 32/8, 8192, 128, 1024, 4    625 / 560 / 503    2, 32/8, 2011, 128, 512, 4   206 / 214 / 184
 //   1, 8/8, 8192, 256, 2048, 64    832 / 641 / 566    1, 16/16, 4096, 64, 1000, 4  111 / 106 / 93
 template <int DP>
 constexpr int kSinkStages = DP <= 128 ? 2 : 1;

@@ -117,7 +117,8 @@ __device__ inline int dec_kswz(int r) {
 // are numbered one after another, and splits and tiles cut that numbering, so a sequence takes
 // as many workgroups as it has tokens to read, however long it is; only the page lookups and
 // nothing of the arithmetic knows of the gap. On MI355X (B 64, 32/8 heads, D 128, 16-token
-// pages, L~U[512, 32768], window 4096, 4 sinks): SINKFIGURE.
+// pages, L~U[512, 32768], window 4096, 4 sinks) 183 us, 5.9 TB/s of the K and V seen; with every
+// length 16000 193 us, as without sinks (194).
 template <typename Tag, int DP, bool SOFTCAP>
 __global__ __launch_bounds__(kDecThreads, kDecMinBlocks<DP>) void decode_split_kernel(
     const DecodeParams p) {

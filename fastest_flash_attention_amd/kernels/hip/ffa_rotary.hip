@@ -17,6 +17,15 @@
 // and sin are formed once for up to kHeadsMost heads; neighbouring threads take the chunks of
 // a row, then the next token. Few tokens (a decode step) take fewer heads per thread instead,
 // down to one, to have threads enough for the chip.
+//
+// Measured on MI355X (bf16 unless said; S tokens, Hq + Hk heads x D, R turned): 2 x 4096, 32 + 8 x
+// 128, 128: 29 us, 5.7 TB/s; 2 x 4097, 24 + 8 x 80, 40: 17.3 us; 64 x 1, 32 + 8 x 128: 3.5 us.
+//   rows loaded at once 1 / 2 / 4 / 8           29.1 / 29.4 / 29.9 / 31.2 us, fp32 7.5 / 7.2 / 7.2 / 7.2
+//   at most 4 / 8 / 16 heads per thread         31.0 / 29.9 / 29.6 us, D 80 17.9 / 18.1 / 17.3
+//   64 / 128 / 256 / 1024 k threads wanted      29.8 / 29.5 / 29.9 / 31.4 us, fp32 7.7 / 8.5 / 7.2 / 8.7
+// Nontemporal stores take 30 us where ordinary ones take 37 (inputs and outputs both cold), but
+// the attention that reads the rows next loses more (rotary and attention together, S 4 x 1024:
+// 68 us against 64), and rows of 160 bytes take 32 us against 17.
 
 #include <type_traits>
 
@@ -27,8 +36,8 @@ namespace ffa {
 namespace {
 
 constexpr int kRotThreads = 256;
-constexpr int kHeadsMost = 8;     // heads that share a thread's cos and sin
-constexpr int kHeadsAtOnce = 4;   // rows whose loads are issued together
+constexpr int kHeadsMost = 16;     // heads that share a thread's cos and sin
+constexpr int kHeadsAtOnce = 2;   // rows whose loads are issued together
 constexpr int64_t kThreadsWanted = 256 * 1024;  // four waves per SIMD
 
 struct Rot32Tag {};

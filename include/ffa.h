@@ -583,8 +583,8 @@ int ffa_paged_copy(const ffa_paged_copy_args* args, void* stream);
  * 8; every tensor is 16-byte aligned with batch/head/seq strides multiples of 8
  * elements (FFA_ERR_MISALIGNED) and seq strides below 2^24 elements. The workspace
  * (16-byte aligned, ffa_attn_bwd_workspace_bytes()) holds per-row statistics; the
- * call overwrites all of it. Three kernels, no atomics: results do not depend on
- * scheduling.
+ * call overwrites all of it. Three kernels, up to four more for sums of parts and for
+ * sinks, no atomics: results do not depend on scheduling.
  */
 typedef struct ffa_attn_bwd_args {
   const void* dout;
