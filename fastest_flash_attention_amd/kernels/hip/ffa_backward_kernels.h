@@ -807,7 +807,8 @@ __global__ __launch_bounds__(kThreads, kBwdMinBlocks<DP>) void bwd_dq_kernel(con
   const int n_win = kv_hi > kv_lo ? (kv_hi + BN - 1) / BN - t_begin : 0;
   // tiles of sinks ahead of the window's
   constexpr bool SINK = kSinks<Tag>;
-  const int n_s = SINK ? min((max(min(p.sinks, kv_hi), 0) + BN - 1) / BN, t_begin) : 0;
+  // (all of theirs where the rows' window holds no key)
+  const int n_s = SINK ? min((max(min(p.sinks, kv_hi), 0) + BN - 1) / BN, n_win > 0 ? t_begin : kMaxPos) : 0;
   const int nt = n_s + n_win;
   auto tile_at = [&](int i) { return SINK && i < n_s ? i : t_begin + (i - n_s); };
 
@@ -1851,7 +1852,8 @@ __global__ __launch_bounds__(kThreads, kF32mDqBlocks<DP>) void bwd_f32m_dq_kerne
   const int t_lo = kv_lo / kM32;
   const int n_win = kv_hi > kv_lo ? (kv_hi + kM32 - 1) / kM32 - t_lo : 0;
   // tiles of sinks ahead of the window's
-  const int n_s = SINK ? min((max(min(p.sinks, kv_hi), 0) + kM32 - 1) / kM32, t_lo) : 0;
+  // (all of theirs where the rows' window holds no key)
+  const int n_s = SINK ? min((max(min(p.sinks, kv_hi), 0) + kM32 - 1) / kM32, n_win > 0 ? t_lo : kMaxPos) : 0;
   const int nt = n_s + n_win;
   auto first_key = [&](int t) { return (SINK && t < n_s ? t : t_lo - n_s + t) * kM32; };
 

@@ -217,8 +217,9 @@ __global__ __launch_bounds__((64 * NW), (kMinBlocks<DP, SOFTCAP> * 4 / NW)) void
   const int kv_hi = p.causal ? min(Skv, ql_abs + 1) : Skv;
   const int t_begin = kv_lo / BN;
   const int nt = kv_hi > kv_lo ? (kv_hi + BN - 1) / BN - t_begin : 0;
-  // tiles of sinks ahead of the window's (a split launch gives them ranges of their own)
-  const int n_s = SINK && !SPLIT ? min((max(min(sinks, kv_hi), 0) + BN - 1) / BN, t_begin) : 0;
+  // tiles of sinks ahead of the window's, or all of theirs where the rows' window holds no key (a
+  // split launch gives them ranges of their own)
+  const int n_s = SINK && !SPLIT ? min((max(min(sinks, kv_hi), 0) + BN - 1) / BN, nt > 0 ? t_begin : kMaxPos) : 0;
 
   const int qw0 = q0 + wave * 32;
   int qrow = qw0 + l32;      // this lane's query row, and its head's offset from h (packed)
@@ -1188,8 +1189,8 @@ __global__ __launch_bounds__(kThreads, 1) void prefill_f32_kernel(const PrefillP
   const int kv_hi = p.causal ? min(Skv, ql_abs + 1) : Skv;
   const int t_begin = kv_lo / kF32BN;
   const int nt = kv_hi > kv_lo ? (kv_hi + kF32BN - 1) / kF32BN - t_begin : 0;
-  // tiles of sinks ahead of the window's
-  const int n_s = SINK ? min((max(min(p.sinks, kv_hi), 0) + kF32BN - 1) / kF32BN, t_begin) : 0;
+  // tiles of sinks ahead of the window's, or all of theirs where the rows' window holds no key
+  const int n_s = SINK ? min((max(min(p.sinks, kv_hi), 0) + kF32BN - 1) / kF32BN, nt > 0 ? t_begin : kMaxPos) : 0;
 
   const int qw0 = q0 + wave * 32;
   const int qrow = qw0 + l32;
@@ -1387,8 +1388,8 @@ __global__ __launch_bounds__(kThreads, kF32SplitBlocks<DP>) void prefill_f32_spl
   const int kv_hi = p.causal ? min(Skv, ql_abs + 1) : Skv;
   const int t_lo = kv_lo / kF32BN;
   const int n_win = kv_hi > kv_lo ? (kv_hi + kF32BN - 1) / kF32BN - t_lo : 0;
-  // tiles of sinks ahead of the window's
-  const int n_s = SINK ? min((max(min(p.sinks, kv_hi), 0) + kF32BN - 1) / kF32BN, t_lo) : 0;
+  // tiles of sinks ahead of the window's, or all of theirs where the rows' window holds no key
+  const int n_s = SINK ? min((max(min(p.sinks, kv_hi), 0) + kF32BN - 1) / kF32BN, n_win > 0 ? t_lo : kMaxPos) : 0;
   const int nt = SINK ? n_s + n_win : n_win;
   auto first_key = [&](int t) { return (SINK && t < n_s ? t : t_lo - n_s + t) * kF32BN; };
   const uint64_t* kmask_row =

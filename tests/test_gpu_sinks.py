@@ -73,6 +73,42 @@ def test_forward(case):
     ref.check(lse, r, "lse", str(case))
 
 
+PAST = [
+    # B, Hq, Hkv, S, Skv, D, dtype, causal, window, sinks, softcap: the last rows' windows lie past
+    # the keys, in the tile of the last sinks or behind it
+    (1, 2, 1, 418, 5, 64, BF16, True, 7, 8, None),
+    (2, 2, 2, 475, 225, 40, FP16, True, 4, 363, None),
+    (1, 4, 1, 361, 1, 128, BF16, True, 109, 5, 20.0),
+    (1, 2, 1, 431, 195, 136, BF16, True, 33, 226, None),
+    (1, 2, 1, 300, 114, 256, FP16, False, 11, 146, None),
+    (1, 2, 1, 300, 300, 128, BF16, False, 1, 3, None),
+    (1, 2, 1, 500, 130, 128, BF16, True, 30, 129, None),
+    (1, 3, 1, 113, 70, 64, FP32, True, 3, 386, 20.0),
+    (1, 2, 1, 418, 5, 128, FP32, True, 7, 8, None),
+    (1, 2, 1, 150, 20, 192, FP32, True, 7, 8, None),
+    (64, 32, 32, 200, 5, 32, FP32, True, 7, 4, None),  # the 128-row fp32 kernel
+]
+
+
+@pytest.mark.parametrize("case", PAST, ids=[str(i) for i in range(len(PAST))])
+def test_rows_past_the_keys(case):
+    """More rows than keys: rows whose window holds no key see the sinks alone."""
+    require_gpu()
+    B, Hq, Hkv, S, Skv, D, dt, causal, W, N, cap = case
+    q, k, v = _qkv(B, Hq, Hkv, S, Skv, D, dt)
+    do = seeded((B, Hq, S, D), dt, 9).cuda()
+    ours, theirs = _opt(causal, W, N, cap)
+    say(f"sinks past the keys {case}")
+    o, lse = ffa.fastest_flash_attn_forward(q, k, v, num_kv_heads=Hkv, return_lse=True, **ours)
+    grads = ffa.fastest_flash_attn_backward(do, q, k, v, o, lse, **ours)
+    b = slice(B - 1, B)
+    r = ref.batch(q[b], k[b], v[b], dout=do[b], **theirs)
+    ref.check(o[b], r, "o", str(case))
+    ref.check(lse[b], r, "lse", str(case))
+    for name, g in zip(("dq", "dk", "dv"), grads):
+        ref.check(g[b], r, name, str(case))
+
+
 def test_large_fp32_grid():
     """The 128-row fp32 kernel (2048 workgroups or more)."""
     require_gpu()
