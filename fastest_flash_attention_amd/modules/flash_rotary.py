@@ -42,15 +42,19 @@ class FastestFlashRotary(nn.Module):
         if magnitude is None:
             magnitude = yarn_magnitude(factor) if scaling == "yarn" else 1.0
         self.magnitude = magnitude
+        self._made_with = dict(rotary_dim=rotary_dim, base=base, scaling=scaling, factor=factor,
+                               original_max_position=original_max_position)
         self.inv_freq = rotary_frequencies(
-            rotary_dim, base, scaling=scaling, factor=factor,
-            original_max_position=original_max_position,
-            device=torch.empty(0).device if device is None else device)
+            **self._made_with, device=torch.empty(0).device if device is None else device)
 
     def _apply(self, fn, *args, **kwargs):
         # follow the module to its device, not to its dtype
         super()._apply(fn, *args, **kwargs)
-        self.inv_freq = self.inv_freq.to(fn(self.inv_freq).device)
+        device = fn(self.inv_freq).device
+        if self.inv_freq.is_meta and device.type != "meta":
+            self.inv_freq = rotary_frequencies(**self._made_with, device=device)
+        else:
+            self.inv_freq = self.inv_freq.to(device)
         return self
 
     def append_options(self, device: torch.device) -> dict:

@@ -239,7 +239,7 @@ def resolve_forward_args(
         compute_dtype = config.compute_dtype
         num_kv_heads = config.num_kv_heads
         return_lse = config.return_lse
-        sink_tokens = config.sink_tokens
+        sink_tokens = getattr(config, "sink_tokens", 0)
 
     sink_tokens = int(sink_tokens)
     if sink_tokens < 0:

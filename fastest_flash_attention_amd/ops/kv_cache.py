@@ -605,6 +605,11 @@ class PagedKVCache(PageBook):
         device, P = self.k_pages.device, self.page_size
         if rotary is not None and device.type != "cuda":
             raise RuntimeError(f"the rotation runs on ROCm tensors only; the pools are on {device}")
+        options = rotary.append_options(device) if rotary is not None else {}
+        if q is not None and (q.dtype != self.k_pages.dtype or q.device != device or q.dim() != k.dim()
+                              or (q.size(0), *q.shape[2:]) != (k.size(0), *k.shape[2:])):
+            raise ValueError(f"q {tuple(q.shape)}, {q.dtype} on {q.device} does not match k "
+                             f"{tuple(k.shape)} and pools of {self.k_pages.dtype} on {device}")
         known = [self.sequences.get(s) or {"page_table": [], "len": 0} for s in seq_ids]
         need = self._pages_to_own(known) if n and self._owners else 0
         need += sum(max(0, -(-(s["len"] + n) // P) - len(s["page_table"])) for s in known)
@@ -617,6 +622,7 @@ class PagedKVCache(PageBook):
                 self.append_tokens(s, k[i].reshape(self.num_heads, n, -1), v[i].reshape(self.num_heads, n, -1))
             return None
         dt = self.k_pages.dtype
+        _lib.dtype_code(dt, allow_fp32=True)
         k, v = k.to(device, dt), v.to(device, dt)
         if self._owners:
             self._own_last_pages(known)
@@ -626,8 +632,7 @@ class PagedKVCache(PageBook):
                 seq["page_table"].append(self.allocate_page())
         tables, at = device_tables([s["page_table"] for s in known], [s["len"] for s in known], device)
         out = fastest_flash_paged_append(
-            k, v, self.k_pages, self.v_pages, tables, at, q=q,
-            **(rotary.append_options(device) if rotary is not None else {}))
+            k, v, self.k_pages, self.v_pages, tables, at, q=q, **options)
         for seq in known:
             seq["len"] += n
         return out

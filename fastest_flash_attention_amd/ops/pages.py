@@ -168,10 +168,12 @@ class PageBook:
         seq = self._sequence(src_id)
         if dst_id in self.sequences:
             raise ValueError(f"sequence {dst_id} exists already")
-        for page in seq["page_table"]:
+        # (pages past the tokens, of an append that failed, stay the first one's: both would write there)
+        table = seq["page_table"][:-(-seq["len"] // self.page_size)]
+        for page in table:
             if page >= 0:
                 self._owners[page] = self._owners.get(page, 1) + 1
-        self.sequences[dst_id] = {"page_table": list(seq["page_table"]), "len": seq["len"]}
+        self.sequences[dst_id] = {"page_table": table, "len": seq["len"]}
 
     def truncate_sequence(self, seq_id: int, length: int) -> None:
         """Keep the first ``length`` tokens of a sequence; pages behind them are released."""

@@ -304,3 +304,21 @@ def test_gpu_refusals():
                       ((q, q, pool.transpose(1, 2), pool, bt, at), ValueError)):
         with pytest.raises(err):
             ffa.fastest_flash_paged_append(*args)
+
+
+def test_refused_append_changes_nothing():
+    """A query or rotation that does not fit is refused before pages are taken."""
+    require_gpu()
+    say("refused append")
+    cache = ffa.PagedKVCache(max_pages=6, page_size=4, num_heads=2, head_dim=16, dtype=torch.bfloat16,
+                             device="cuda")
+    kv = torch.ones(2, 2, 4, 16, dtype=torch.bfloat16, device="cuda")
+    rot = ffa.FastestFlashRotary(16, device="cuda")
+    cache.append_batch([0, 1], kv, kv)
+    before = {s: (list(q["page_table"]), q["len"]) for s, q in cache.sequences.items()}, list(cache.free_pages)
+    for q in (kv.float(), kv[:, :, :3], kv[:1], kv.cpu(), kv[..., :8]):
+        with pytest.raises(ValueError, match="does not match"):
+            cache.append_batch([0, 5], kv, kv, q=q, rotary=rot)
+    with pytest.raises(RuntimeError, match="rotary module is on"):
+        cache.append_batch([0, 5], kv, kv, rotary=ffa.FastestFlashRotary(16))
+    assert before == ({s: (q["page_table"], q["len"]) for s, q in cache.sequences.items()}, cache.free_pages)

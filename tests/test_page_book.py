@@ -123,6 +123,18 @@ def test_full_pages_stay_shared():
     _invariants(cache)
 
 
+def test_fork_leaves_pages_without_tokens_to_the_first():
+    """A page taken ahead of its tokens (an append that failed) is not written by both."""
+    cache = _cache()
+    cache.append_tokens(0, *_tokens(4, 1))
+    cache.sequences[0]["page_table"].append(cache.allocate_page())
+    cache.fork_sequence(0, 1)
+    cache.append_tokens(0, *_tokens(1, 50))
+    cache.append_tokens(1, *_tokens(1, 60))
+    _check(cache, {0: [1, 2, 3, 4, 50], 1: [1, 2, 3, 4, 60]})
+    _invariants(cache)
+
+
 def test_out_of_pages_appends_nothing():
     cache = _cache(pages=3)
     cache.append_tokens(0, *_tokens(5, 1))

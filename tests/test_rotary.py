@@ -63,6 +63,15 @@ def test_module_keeps_64_bits():
     assert m.inv_freq.device.type == "meta" and m.inv_freq.dtype == torch.float64
 
 
+def test_module_made_without_memory():
+    """Made on the meta device, the frequencies are there once the module has memory."""
+    with torch.device("meta"):
+        m = ffa.FastestFlashRotary(32, scaling="linear", factor=4.0)
+    assert m.inv_freq.is_meta
+    m.to_empty(device="cpu")
+    assert torch.equal(m.inv_freq, ffa.rotary_frequencies(32, scaling="linear", factor=4.0))
+
+
 def test_entry_points_refuse_host_tensors():
     q = torch.zeros(1, 2, 3, 8)
     f = ffa.rotary_frequencies(8)
