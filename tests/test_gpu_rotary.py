@@ -58,7 +58,7 @@ CASES = [
     (2, 5, 1, 9, 7, 4, FP16, True),        # rows of 14 bytes
     (2, 3, 3, 17, 33, 10, FP32, False),
     (2, 3, 3, 17, 64, 64, FP32, True),
-    (1, 40, 8, 700, 128, 64, BF16, False),  # enough rows for eight heads a thread
+    (1, 40, 8, 700, 128, 64, BF16, False),  # several heads a thread
     (1, 2, 2, 300, 256, 256, FP16, True),
 ]
 
@@ -304,6 +304,48 @@ def test_gpu_refusals():
                       ((q, q, pool.transpose(1, 2), pool, bt, at), ValueError)):
         with pytest.raises(err):
             ffa.fastest_flash_paged_append(*args)
+
+
+def test_offsets_past_32_bits():
+    """Rows and pages past 4 GiB of a tensor or pool: the same as those at its beginning."""
+    require_gpu()
+    say("rotary past 4 GiB")
+    S, H, D = 270000, 64, 128
+    q = torch.empty(1, S, H, D, dtype=BF16, device="cuda").transpose(1, 2)
+    tail = seeded((1, H, 37, D), BF16, 1).cuda()
+    q[:, :, :-37].zero_()
+    q[:, :, -37:] = tail
+    assert q.numel() * 2 > 1 << 32
+    freq = ffa.rotary_frequencies(D, device="cuda")
+    got, _ = ffa.fastest_flash_rotary(q, None, freq)
+    want, _ = ffa.fastest_flash_rotary(tail, None, freq, q_offset=S - 37)
+    assert torch.equal(got[:, :, -37:], want) and not got[:, :, :-37].any()
+    del q, got
+    P, page, Hkv = 34000, 64, 8
+    pools = [torch.empty(P, Hkv, page, D, dtype=BF16, device="cuda") for _ in range(2)]
+    small = [torch.empty(4, Hkv, page, D, dtype=BF16, device="cuda") for _ in range(2)]
+    assert pools[0].numel() * 2 > 1 << 32
+    k, v = (seeded((1, Hkv, 100, D), BF16, s).cuda() for s in (2, 3))
+    at = torch.tensor([40], dtype=torch.int32, device="cuda")
+    far = torch.tensor([[P - 2, 3, P - 1]], dtype=torch.int32, device="cuda")
+    near = torch.tensor([[2, 0, 1]], dtype=torch.int32, device="cuda")
+    for x in (*pools, *small):
+        x[-4:].zero_()
+        x[:4].zero_()
+    say("append, copy and decode past 4 GiB")
+    ffa.fastest_flash_paged_append(k, v, *pools, far, at, inv_freq=freq)
+    ffa.fastest_flash_paged_append(k, v, *small, near, at, inv_freq=freq)
+    ffa.fastest_flash_copy_pages(*pools, [P - 2, 3], [P - 3, P - 4])
+    ffa.fastest_flash_copy_pages(*small, [2], [3])
+    for a, b in zip(pools, small):
+        assert torch.equal(a[P - 2], b[2]) and torch.equal(a[3], b[0]) and torch.equal(a[P - 1], b[1])
+        assert torch.equal(a[P - 3], b[3]) and torch.equal(a[P - 4], b[0])
+    lens = torch.tensor([140], dtype=torch.int32, device="cuda")
+    x = seeded((1, 16, D), BF16, 4).cuda()
+    how = dict(sliding_window=50, sink_tokens=45, max_context_len=140)
+    a, _ = ffa.fastest_flash_paged_decode(x, *pools, far, lens, **how)
+    b, _ = ffa.fastest_flash_paged_decode(x, *small, near, lens, **how)
+    assert torch.equal(a, b) and a.any()
 
 
 def test_refused_append_changes_nothing():
