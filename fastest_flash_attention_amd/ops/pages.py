@@ -135,17 +135,24 @@ class PageBook:
         """Before tokens are appended to ``seqs``: a copy of its own, of a last page that is
         not full and shared, for each of them but the page's last owner. The caller has seen
         to the free pages (``_pages_to_own``)."""
-        src, dst = [], []
+        owners: Dict[int, int] = {}  # of the shared pages, less those that get a copy
+        moves = []
         for seq in seqs:
             at, part = divmod(seq["len"], self.page_size)
-            if part and seq["page_table"][at] in self._owners:
-                page = seq["page_table"][at]
-                seq["page_table"][at] = self.allocate_page()
-                self._release(page)
-                src.append(page)
-                dst.append(seq["page_table"][at])
-        if src:
-            self._copy(src, dst)
+            page = seq["page_table"][at] if part else -1
+            if owners.setdefault(page, self._owners.get(page, 1)) > 1:
+                owners[page] -= 1
+                moves.append((seq, at, page, self.allocate_page()))
+        if not moves:
+            return
+        try:
+            self._copy([m[2] for m in moves], [m[3] for m in moves])
+        except Exception:
+            self.free_pages[:0] = [m[3] for m in moves]
+            raise
+        for seq, at, page, own in moves:
+            seq["page_table"][at] = own
+            self._release(page)
 
     def _pages_to_own(self, seqs: Sequence[dict]) -> int:
         """Free pages that ``_own_last_pages`` takes."""

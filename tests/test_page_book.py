@@ -112,6 +112,24 @@ def test_fork_copies_the_last_page_once():
     _invariants(cache)
 
 
+def test_failed_copy_leaves_the_page_shared():
+    cache = _cache()
+    cache.append_tokens(0, *_tokens(6, 1))
+    cache.fork_sequence(0, 1)
+    before = {s: list(q["page_table"]) for s, q in cache.sequences.items()}, list(cache.free_pages)
+
+    def fails(src, dst):
+        raise RuntimeError("no copy")
+    cache._copy = fails
+    with pytest.raises(RuntimeError, match="no copy"):
+        cache.append_tokens(1, *_tokens(1, 50))
+    assert before == ({s: q["page_table"] for s, q in cache.sequences.items()}, cache.free_pages)
+    del cache._copy
+    cache.append_tokens(1, *_tokens(1, 50))
+    _check(cache, {0: [1, 2, 3, 4, 5, 6], 1: [1, 2, 3, 4, 5, 6, 50]})
+    _invariants(cache)
+
+
 def test_full_pages_stay_shared():
     cache = _cache()
     cache.append_tokens(0, *_tokens(8, 1))
