@@ -273,11 +273,11 @@ def fastest_flash_paged_decode(
         tokens_per_split = _auto_tokens_per_split(B, Hkv, span)
 
     lib = _lib.load()
-    out = torch.empty((B, Hq, D), dtype=q3.dtype, device=q3.device)
-    lse = torch.empty((B, Hq), dtype=torch.float32, device=q3.device) if return_lse else None
+    out = q3.new_empty((B, Hq, D))
+    lse = q3.new_empty((B, Hq), dtype=torch.float32) if return_lse else None
     need = int(lib.ffa_paged_decode_workspace_bytes(B, Hq, D, span, tokens_per_split))
     if workspace is None or workspace.numel() * workspace.element_size() < need:
-        workspace = torch.empty(max(need, 4), dtype=torch.uint8, device=q3.device)
+        workspace = q3.new_empty(max(need, 4), dtype=torch.uint8)
 
     a = _lib.PagedDecodeArgs()
     a.q = q3.data_ptr()
@@ -343,12 +343,12 @@ def fastest_flash_paged_append(
     read from the device, so the call can be captured into a graph. No gradients.
     """
     one = k.dim() == 3
-    if one:
-        k, v = k.unsqueeze(2), v.unsqueeze(2) if v.dim() == 3 else v
-        q = q.unsqueeze(2) if q is not None and q.dim() == 3 else q
-    if k.dim() != 4 or k.shape != v.shape:
+    if k.dim() not in (3, 4) or k.shape != v.shape:
         raise ValueError("k and v must both be [B, Hkv, n, D] or [B, Hkv, D]")
-    B, Hkv, n, D = k.shape
+    if one:
+        (B, Hkv, D), n = k.shape, 1
+    else:
+        B, Hkv, n, D = k.shape
     if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
         raise ValueError("k_pages / v_pages must both be [num_pages, Hkv, page_size, D]")
     if k_pages.size(1) != Hkv or k_pages.size(3) != D:
@@ -361,12 +361,14 @@ def fastest_flash_paged_append(
     if q is not None:
         if inv_freq is None:
             raise ValueError("q is rotated only: it needs inv_freq")
-        if q.dim() != 4 or (q.size(0), q.size(2), q.size(3)) != (B, n, D):
+        if one and q.dim() == 4 and q.size(2) == 1:
+            q = q[:, :, 0]
+        if q.dim() != k.dim() or q.size(0) != B or q.size(-1) != D or not (one or q.size(2) == n):
             raise ValueError(f"q {tuple(q.shape)} does not match k {tuple(k.shape)}")
     if block_tables.dim() != 2 or block_tables.size(0) != B:
         raise ValueError(f"block_tables must be [B, max_blocks] with B {B}")
     for name, t in (("positions", positions), ("counts", counts)):
-        if t is not None and tuple(t.shape) != (B,):
+        if t is not None and (t.dim() != 1 or t.size(0) != B):
             raise ValueError(f"{name} must be [B] with B {B}")
     if block_tables.dtype != torch.int32 or positions.dtype != torch.int32 or (
             counts is not None and counts.dtype != torch.int32):
@@ -388,16 +390,18 @@ def fastest_flash_paged_append(
         a.rotary_dim = 2 * inv_freq.numel()
     a.magnitude = check_magnitude(magnitude)
     a.interleaved = 1 if interleaved else 0
-    k, v = (t if D == 1 or t.stride(3) == 1 else t.contiguous() for t in (k, v))
+    k = k if D == 1 or k.stride(-1) == 1 else k.contiguous()
+    v = v if D == 1 or v.stride(-1) == 1 else v.contiguous()
     out = None
+    m = k.dim() - 1  # strides (one token a sequence: 0 between tokens)
     if q is not None:
-        q, out, a.q_stride[:], a.q_out_stride[:] = in_and_out(q)
+        q, out, a.q_stride[:m], a.q_out_stride[:m] = in_and_out(q)
         a.q, a.q_out, a.heads_q = q.data_ptr(), out.data_ptr(), q.size(1)
     block_tables, positions = block_tables.contiguous(), positions.contiguous()
     counts = counts.contiguous() if counts is not None else None
     a.k_pages, a.v_pages = k_pages.data_ptr(), v_pages.data_ptr()
     a.k_new, a.v_new = k.data_ptr(), v.data_ptr()
-    a.k_new_stride[:], a.v_new_stride[:] = k.stride()[:3], v.stride()[:3]
+    a.k_new_stride[:m], a.v_new_stride[:m] = k.stride()[:m], v.stride()[:m]
     a.block_tables, a.positions = block_tables.data_ptr(), positions.data_ptr()
     a.counts = counts.data_ptr() if counts is not None else None
     a.block_table_stride = block_tables.size(1)
@@ -408,8 +412,6 @@ def fastest_flash_paged_append(
         _lib.launch(_lib.load().ffa_paged_append_batch, a, device)
     elif out is not None and out.numel():
         raise ValueError("the page pools or block_tables are empty")
-    if out is not None and one:
-        out = out.squeeze(2)
     return out
 
 

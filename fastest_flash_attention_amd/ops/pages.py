@@ -59,7 +59,7 @@ def fastest_flash_copy_pages(
                            f"on {k_pages.device}")
     device = k_pages.device
     num_pages = k_pages.size(0)
-    page_bytes = k_pages[0].numel() * k_pages.element_size() if num_pages else 0
+    page_bytes = k_pages.numel() // num_pages * k_pages.element_size() if num_pages else 0
     if page_bytes % 2:
         raise TypeError(f"pages of {page_bytes} bytes are not supported")
     on_device = [isinstance(x, torch.Tensor) and x.is_cuda for x in (src, dst)]

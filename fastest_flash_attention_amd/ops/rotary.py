@@ -100,17 +100,17 @@ def check_magnitude(magnitude: float) -> float:
 
 
 def in_and_out(t: torch.Tensor):
-    """The tensor as the kernel reads it, its output, and their strides of batch, head and token."""
+    """The tensor as the kernel reads it, its output, and their strides ahead of the last dim's."""
     stride = t.stride()
-    if stride[3] != 1 and t.size(3) > 1:
+    if stride[-1] != 1 and t.size(-1) > 1:
         t = t.contiguous()
         stride = t.stride()
     out = torch.empty_like(t)
     out_stride = out.stride()
-    if out_stride[3] != 1 and t.size(3) > 1:
+    if out_stride[-1] != 1 and t.size(-1) > 1:
         out = torch.empty(t.shape, dtype=t.dtype, device=t.device)
         out_stride = out.stride()
-    return t, out, stride[:3], out_stride[:3]
+    return t, out, stride[:-1], out_stride[:-1]
 
 
 def _rotate(q: Optional[torch.Tensor], k: Optional[torch.Tensor], inv_freq: torch.Tensor,
