@@ -23,9 +23,10 @@
 //   rows loaded at once 1 / 2 / 4 / 8           29.1 / 29.4 / 29.9 / 31.2 us, fp32 7.5 / 7.2 / 7.2 / 7.2
 //   at most 4 / 8 / 16 heads per thread         31.0 / 29.9 / 29.6 us, D 80 17.9 / 18.1 / 17.3
 //   64 / 128 / 256 / 1024 k threads wanted      29.8 / 29.5 / 29.9 / 31.4 us, fp32 7.7 / 8.5 / 7.2 / 8.7
-// Nontemporal stores take 30 us where ordinary ones take 37 (inputs and outputs both cold), but
-// the attention that reads the rows next loses more (rotary and attention together, S 4 x 1024:
-// 68 us against 64), and rows of 160 bytes take 32 us against 17.
+// With inputs and outputs both cold it takes 37 us. Nontemporal stores take 30 then, but the
+// attention that reads the rows next loses more (rotary and attention together, 4 x 1024 tokens: 68 us
+// against 64), and rows of 160 bytes take 32 us against 17. Nontemporal loads: 33 us cold, but 33
+// against 29 warm and 31 against 17 with rows of 160 bytes.
 
 #include <type_traits>
 
