@@ -265,7 +265,8 @@ __device__ inline void load_lds16(const void* src, void* lds_base) {
 // spilled base with v_readlane right before this asm, the load goes to a wrong address. GUARD
 // copies the base in the asm (a scalar move waits for the VALU, and the load for the move): for
 // kernels that spill their bases. The others are held to the distance by
-// tests/test_asm_hazards.py.
+// tests/test_asm_hazards.py. The load must also stay one wait state behind the scalar move that
+// sets M0: the asm's own s_nop, or GUARD's move.
 template <bool GUARD = false>
 __device__ inline void load_lds16_async(const void* base, uint32_t voff, uint32_t lds_base) {
   if constexpr (GUARD) {
@@ -275,7 +276,7 @@ __device__ inline void load_lds16_async(const void* base, uint32_t voff, uint32_
                  : "v"(voff), "s"(base), "{m0}"(__builtin_amdgcn_readfirstlane(lds_base))
                  : "memory");
   } else {
-    asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(base),
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(base),
                  "{m0}"(__builtin_amdgcn_readfirstlane(lds_base))
                  : "memory");
   }
@@ -283,7 +284,7 @@ __device__ inline void load_lds16_async(const void* base, uint32_t voff, uint32_
 
 // Same, with a per-lane 64-bit address (sources that need not share a 4 GiB window).
 __device__ inline void load_lds16_async(const void* src, uint32_t lds_base) {
-  asm volatile("global_load_lds_dwordx4 %0, off" ::"v"(src),
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src),
                "{m0}"(__builtin_amdgcn_readfirstlane(lds_base))
                : "memory");
 }

@@ -4,7 +4,8 @@ instruction that wrote it (CPU, no GPU needed: the built code objects are disass
 The hardware does not wait there. The compiler keeps the distance for loads that it emits, not for
 those in inline asm: a kernel whose base address was a spilled SGPR, restored by v_readlane right
 before the asm load, read a wrong address. Kernels that spill their bases copy them inside the asm
-(ffa_common.h); this test holds all others to the distance.
+(ffa_common.h); this test holds all others to the distance. A load into LDS must also stay one wait
+state behind the scalar write of M0, which holds its LDS address.
 """
 
 from __future__ import annotations
@@ -70,6 +71,25 @@ def hazards(lines):
     return found
 
 
+def m0_hazards(lines):
+    """Loads into LDS right behind a scalar write of M0."""
+    found, before = [], ""
+    for line in lines:
+        text = line.split("//")[0].strip()
+        if not text:
+            continue
+        if "load_lds" in text and re.match(r"s_\S+ m0,", before):
+            found.append((before, text))
+        before = text
+    return found
+
+
+def test_scanner_finds_a_planted_m0_hazard():
+    load = "global_load_lds_dwordx4 v1, s[4:5]"
+    assert m0_hazards(["s_mov_b32 m0, s3", "", load]) == [("s_mov_b32 m0, s3", load)]
+    assert not m0_hazards(["s_mov_b32 m0, s3", "s_nop 0", load])
+
+
 def test_scanner_finds_planted_hazards():
     def snippet(*between):
         return ["0000 <k>:", "v_readlane_b32 s1, v167, 57", *between, "global_load_lds_dwordx4 v120, s[0:1]"]
@@ -96,6 +116,6 @@ def test_no_kernel_reads_a_fresh_sgpr(tmp_path):
     for f in images:
         out = subprocess.run([OBJDUMP, "-d", f], check=True, capture_output=True, text=True, cwd=tmp_path).stdout
         loads += out.count("global_load_lds_dwordx4")
-        found += hazards(out.splitlines())
+        found += hazards(out.splitlines()) + m0_hazards(out.splitlines())
     assert loads > 1000
     assert not found, "\n".join(str(x) for x in found[:20])
