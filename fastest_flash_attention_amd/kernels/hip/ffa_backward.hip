@@ -18,6 +18,12 @@ size_t attn_bwd_workspace_bytes(int32_t batch, int32_t heads_q, int32_t seqlen_q
 
 namespace {
 
+// Whether the dK/dV kernel runs with two halves (its comment has the rule and what it measured):
+// calls with sinks, at most a workgroup per CU, sweeps (the longest: `most` tiles) long enough.
+bool pair_waves(const BwdParams& p, int64_t units, int64_t most) {
+  return p.sinks > 0 && p.D <= 128 && p.n_part_s == 1 && units * p.n_kt <= 256 && (p.D <= 64 || most >= 10);
+}
+
 // Cuts the dK/dV sweeps of a launch that its heaviest workgroup would hold up: sets n_part,
 // part_len and the key tiles cut, returns the bytes of the partials (0: no sweep is cut). A part is 1.5 times
 // an even share of the work over the chip's slots (two workgroups per CU up to head_dim
@@ -37,6 +43,7 @@ namespace {
 //   2, 16/4, 3000, 128, window 500, 256 sinks     202 / 202, 218
 //   4, 32/8, 4096, 64, window 256, 128 sinks      415 / 415, 333
 size_t plan_dkv_parts(BwdParams& p, int32_t dtype) {
+  p.pair = 0;
   p.n_part = p.n_part_s = 1;
   p.part_len = p.part_len_s = 0x7fffffff;
   const int64_t units = static_cast<int64_t>(p.B) * p.Hkv;
@@ -64,6 +71,7 @@ size_t plan_dkv_parts(BwdParams& p, int32_t dtype) {
     bytes += static_cast<size_t>(units) * p.n_skt * p.n_part_s * tile_bytes;
   }
   len = even < 16 ? 16 : even;
+  p.pair = pair_waves(p, units, most) ? 1 : 0;
   if (!few || 2 * most <= 5 * len) return bytes;
   if (most > 16 * len) len = (most + 15) / 16;  // at most 16 parts
   p.n_part = static_cast<int>((most + len - 1) / len);

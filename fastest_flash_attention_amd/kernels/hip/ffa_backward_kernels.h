@@ -96,6 +96,7 @@ struct BwdParams {
   float* part_s;  // [B * Hkv][n_skt][n_part_s][128 keys][D + Dv]
   int sink0, n_skb, n_part_k, part_len_k;
   float* part_k;  // [B * Hkv][n_skb][n_part_k][32 keys][2 D] (n_part_k > 1)
+  int pair;  // the dK/dV kernel with two halves (host only)
 };
 
 }  // namespace bwd
@@ -349,12 +350,25 @@ constexpr int kBwdMinBlocks = DP <= 128 ? 2 : 1;
 // the rule and what it measured). A variant of its own: the part's bounds cost the uncut
 // kernel 2-4 % (8 % at head_dim 64), and at head_dim 256 they spill.
 //
+// PAIR: eight waves, two halves of four that hold the same keys and take row tiles in turn, from
+// LDS buffers of their own; the second half's sums are added to the first's in LDS at the end. For
+// grids of at most one workgroup per CU, whose four waves leave the matrix units idle between
+// dependent steps (28 % busy at the first shape below): as many waves as two workgroups of a
+// larger grid, and no partial sums in memory. Whole backward on MI355X, us, without / with (B, Hq/Hkv, S, D,
+// window, 4 sinks, bf16; the longest sweep in row tiles):
+//   2, 32/8, 2011, 128, 512    212 / 197 (80)      2, 32/8, 2048, 64, 512   147 / 117 (80)
+//   1, 8/8, 4096, 128, 2000    168 / 152 (67)      1, 8/2, 300, 64, 64      58 / 46 (24)
+//   2, 8/8, 2000, 128, 288     70.4 / 69.2 (13)    2, 8/8, 2000, 64, 288    53 / 49 (13)
+//   2, 8/8, 2000, 128, 96      60.9 / 61.5 (7)     2, 8/8, 2000, 64, 96     44 / 42 (7)
+// so from ten tiles on (pair_waves in ffa_backward.hip), and always up to head_dim 64.
+//
 // SINK (Tag = Sinks<...>): whole tiles of sinks are swept by every row, the others by a window's:
 // S / 32 tiles a head against (W + 128) / 32, by a few workgroups. So they come first in the grid,
 // cut into parts (plan_dkv_parts). The sinks past the last whole tile are left to bwd_sink_kernel:
 // this kernel computes their window's share along with their tile's and does not store it.
-template <typename Tag, int DP, int DV, bool SOFTCAP, bool CUT>
-__global__ __launch_bounds__(kThreads, kBwdMinBlocks<DP>) void bwd_dkdv_kernel(const BwdParams p) {
+template <typename Tag, int DP, int DV, bool SOFTCAP, bool CUT, bool PAIR = false>
+__global__ __launch_bounds__(PAIR ? 2 * kThreads : kThreads, PAIR ? 1 : kBwdMinBlocks<DP>)
+void bwd_dkdv_kernel(const BwdParams p) {
   using S = BShape<DP>;   // Q, K, dK
   using SV = BShape<DV>;  // dO, V, dV
   using E = Elem<Tag>;
@@ -364,13 +378,16 @@ __global__ __launch_bounds__(kThreads, kBwdMinBlocks<DP>) void bwd_dkdv_kernel(c
   constexpr int LPTV = kDkvRows * SV::CPR / kThreads;  // dO tile loads per thread
   static_assert(kDkvRows * S::CPR % kThreads == 0 && kDkvRows * SV::CPR % kThreads == 0,
                 "tile must split evenly");
-  __shared__ __attribute__((aligned(1024))) uint16_t q_lds[2][TILE];
-  __shared__ __attribute__((aligned(1024))) uint16_t do_lds[2][TILE_V];
-  __shared__ __attribute__((aligned(1024))) float st_lds[2][256];  // [0,32) lse2, [32,64) D_i
+  static_assert(!PAIR || (DP == DV && DP <= 128 && !CUT), "what the halves' sum is written for");
+  constexpr int NG = PAIR ? 2 : 1;  // halves of the workgroup, each on row tiles of its own
+  __shared__ __attribute__((aligned(1024))) uint16_t q_lds[2 * NG][TILE];
+  __shared__ __attribute__((aligned(1024))) uint16_t do_lds[2 * NG][TILE_V];
+  __shared__ __attribute__((aligned(1024))) float st_lds[2 * NG][256];  // [0,32) lse2, [32,64) D_i
   __shared__ __attribute__((aligned(1024))) uint16_t v_lds[4][32 * DV];  // each wave's V rows
 
   const int tid = threadIdx.x;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(PAIR ? (tid >> 6) & 3 : tid >> 6);
+  const int half = PAIR ? __builtin_amdgcn_readfirstlane(tid >> 8) : 0;
   const int lane = tid & 63;
   const int l32 = lane & 31;
   const int g = lane >> 5;
@@ -433,7 +450,7 @@ __global__ __launch_bounds__(kThreads, kBwdMinBlocks<DP>) void bwd_dkdv_kernel(c
   u32x4 kreg[S::KS];
   load_row_operand<DP>(p.k + b * p.k_sb + hk * p.k_sh +
                            static_cast<int64_t>(min(key, p.Skv - 1)) * p.k_ss, D, g, kreg);
-  if (wave_live) {
+  if (wave_live && half == 0) {
     const uint16_t* vb = p.v + b * p.v_sb + hk * p.v_sh + static_cast<int64_t>(kw0) * p.v_ss;
 #pragma unroll
     for (int j = 0; j < 32 * SV::CPR / 64; ++j) {
@@ -481,7 +498,14 @@ __global__ __launch_bounds__(kThreads, kBwdMinBlocks<DP>) void bwd_dkdv_kernel(c
   // The next tile to issue is tracked incrementally (head r of the group, tile index
   // qi, running byte pointers) instead of dividing the iteration index.
   int is_r = it_begin > 0 ? it_begin / ntq : 0;
-  int is_qi = it_begin - is_r * ntq;
+  int is_qi = it_begin - is_r * ntq + half;
+  auto wrap = [&]() {  // PAIR: steps of two may pass the end of a head or two
+    while (is_qi >= ntq && is_r < p.ratio) {
+      is_qi -= ntq;
+      ++is_r;
+    }
+  };
+  if constexpr (PAIR) wrap();
   const char* is_qb = nullptr;
   const char* is_db = nullptr;
   int64_t is_ws = 0;
@@ -489,7 +513,7 @@ __global__ __launch_bounds__(kThreads, kBwdMinBlocks<DP>) void bwd_dkdv_kernel(c
   const int64_t do_tile_bytes = static_cast<int64_t>(kDkvRows) * p.do_ss * 2;
   auto is_head = [&]() {
     const int hq = hk * p.ratio + is_r;
-    const int q0 = (CUT ? qt_begin + is_qi : qt_begin) * kDkvRows;
+    const int q0 = (CUT || PAIR ? qt_begin + is_qi : qt_begin) * kDkvRows;
     is_qb = reinterpret_cast<const char*>(p.q + b * p.q_sb + hq * p.q_sh +
                                           static_cast<int64_t>(q0) * p.q_ss);
     is_db = reinterpret_cast<const char*>(p.dout + b * p.do_sb + hq * p.do_sh +
@@ -534,7 +558,11 @@ __global__ __launch_bounds__(kThreads, kBwdMinBlocks<DP>) void bwd_dkdv_kernel(c
       const float* src = ((lane & 8) ? p.di : p.lse2) + is_ws + 4 * (lane & 7);
       load_lds16_async(src, lds_addr(&st_lds[buf][0]));
     }
-    if (++is_qi == ntq) {
+    if constexpr (PAIR) {
+      is_qi += 2;
+      wrap();
+      if (is_r < p.ratio) is_head();
+    } else if (++is_qi == ntq) {
       is_qi = 0;
       ++is_r;
       if (is_r < p.ratio) is_head();
@@ -568,14 +596,20 @@ __global__ __launch_bounds__(kThreads, kBwdMinBlocks<DP>) void bwd_dkdv_kernel(c
   }
 
   int cur_qi = is_qi;  // q tile index (within [0, ntq)) of iteration it
-  if (it_end > it_begin) issue(0);
-  for (int it = it_begin; it < it_end; ++it) {
-    const int buf = (it - it_begin) & 1;
+  if (it_end > it_begin + half) issue(2 * half);
+  for (int it = it_begin; it < it_end; it += NG) {  // (halves: tile it + half, both to the last barrier)
+    const int buf = 2 * half + ((it - it_begin) / NG & 1);
     wait_vmcnt0();
     __syncthreads();
-    if (it + 1 < it_end) issue(buf ^ 1);
+    if (it + NG + half < it_end) issue(buf ^ 1);
     const int q0 = (qt_begin + cur_qi) * kDkvRows;
-    if (++cur_qi == ntq) cur_qi = 0;
+    if constexpr (PAIR) {
+      cur_qi += 2;
+      while (cur_qi >= ntq) cur_qi -= ntq;
+      if (it + half >= it_end) continue;
+    } else {
+      if (++cur_qi == ntq) cur_qi = 0;
+    }
     const int q0_abs = p.q_offset + q0;
     if (!wave_live) continue;
     if (p.causal && kw0 > q0_abs + kDkvRows - 1) continue;
@@ -681,6 +715,35 @@ __global__ __launch_bounds__(kThreads, kBwdMinBlocks<DP>) void bwd_dkdv_kernel(c
     }
   }
 
+  if constexpr (PAIR) {  // the second half's sums to the first, in LDS: dK, then dV
+    constexpr int HB = S::DB / 2;  // blocks in q_lds, as many in do_lds
+    static_assert(4 * HB * 16 * 64 * 4 <= 2 * NG * TILE * 2, "half of the blocks fit in q_lds");
+    auto add = [&](f32x16 (&acc)[S::DB]) {
+      __syncthreads();  // tiles, or the sums before, are read
+#pragma unroll
+      for (int db = 0; db < S::DB; ++db) {
+        float* red = reinterpret_cast<float*>(db < HB ? &q_lds[0][0] : &do_lds[0][0]) +
+                     (wave * HB + db % HB) * 16 * 64 + lane;
+        if (half == 1) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) red[64 * r] = acc[db][r];
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int db = 0; db < S::DB; ++db) {
+        const float* red = reinterpret_cast<const float*>(db < HB ? &q_lds[0][0] : &do_lds[0][0]) +
+                           (wave * HB + db % HB) * 16 * 64 + lane;
+        if (half == 0) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[db][r] += red[64 * r];
+        }
+      }
+    };
+    add(dkacc);
+    add(dvacc);
+    if (half == 1) return;
+  }
   if (cut) {
     if (key < p.Skv) {
       int64_t tile = (static_cast<int64_t>(bh) * p.n_cut + (kt - p.cut_first)) * p.n_part + part;
@@ -2009,7 +2072,15 @@ void launch_main(const BwdParams& p, int grid_dkv, int grid_dq, hipStream_t s) {
         }
       }
     }
-    if (!cut) {
+    bool pair = false;
+    if constexpr (kSinks<Tag> && DP <= 128) {
+      pair = !cut && p.pair != 0;
+      if (pair) {
+        hipLaunchKernelGGL((bwd_dkdv_kernel<Tag, DP, DV, SOFTCAP, false, true>), dim3(grid_dkv), dim3(2 * kThreads),
+                           0, s, p);
+      }
+    }
+    if (!cut && !pair) {
       hipLaunchKernelGGL((bwd_dkdv_kernel<Tag, DP, DV, SOFTCAP, false>), dim3(grid_dkv), dim3(kThreads), 0, s, p);
     }
   }
