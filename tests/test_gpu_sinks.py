@@ -9,6 +9,7 @@ import pytest
 import torch
 
 import fastest_flash_attention_amd as ffa
+from fastest_flash_attention_amd.kernels import _lib
 from fastest_flash_attention_amd.ops.attention_forward import launch_prefill, prepare_prefill
 from tests import sinks_ref as ref
 from tests.gpu_util import require_gpu, say, seeded
@@ -318,6 +319,43 @@ def test_backward_q_offset():
                                                 q_offset=off)
         for name, g in zip(("dq", "dk", "dv"), grads):
             ref.check(g, r, name, "offset")
+
+
+@pytest.mark.parametrize("D,dt,N", [(64, BF16, 9), (128, FP16, 9), (128, BF16, 300), (192, BF16, 140),
+                                    (256, BF16, 40), (64, FP32, 40), (192, FP32, 9)])
+def test_backward_without_room_for_parts(D, dt, N, monkeypatch):
+    """With the workspace of the statistics alone no sweep is cut: the same gradients."""
+    require_gpu()
+    q, k, v = _qkv(1, 4, 1, 700, 700, D, dt)
+    do = seeded((1, 4, 700, D), dt, 9).cuda()
+    ours, theirs = _opt(True, 60, N, None)
+    o, lse = ffa.fastest_flash_attn_forward(q, k, v, num_kv_heads=1, return_lse=True, **ours)
+    lib = _lib.load()
+    monkeypatch.setattr(lib, "ffa_attn_bwd_split_workspace_bytes", lambda _: 0)
+    say(f"sinks backward uncut {D} {dt} {N}")
+    grads = ffa.fastest_flash_attn_backward(do, q, k, v, o, lse, **ours)
+    r = ref.batch(q, k, v, dout=do, **theirs)
+    for name, g in zip(("dq", "dk", "dv"), grads):
+        ref.check(g, r, name, "uncut")
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("S,Hq,W", [(1, 2, 1), (31, 1, 7), (33, 1, 7), (65, 3, 40), (96, 5, 60), (450, 7, 333)])
+def test_backward_with_two_halves(D, S, Hq, W):
+    """Sweeps of one tile, of odd and even numbers of them, over heads of one and more tiles: two
+    halves of a workgroup take them in turn, with results that do not change from run to run."""
+    require_gpu()
+    q, k, v = _qkv(2, Hq, 1, S, S, D, BF16)
+    do = seeded((2, Hq, S, D), BF16, 9).cuda()
+    ours, theirs = _opt(True, W, 3, None)
+    say(f"sinks halves {D} {S} {Hq} {W}")
+    o, lse = ffa.fastest_flash_attn_forward(q, k, v, num_kv_heads=1, return_lse=True, **ours)
+    grads = ffa.fastest_flash_attn_backward(do, q, k, v, o, lse, **ours)
+    again = ffa.fastest_flash_attn_backward(do, q, k, v, o, lse, **ours)
+    r = ref.batch(q, k, v, dout=do, **theirs)
+    for name, g, h in zip(("dq", "dk", "dv"), grads, again):
+        ref.check(g, r, name, "halves")
+        assert torch.equal(g, h)
 
 
 def _paged(lens, page, Hkv, D, dt, spare=3, seed=0):
